@@ -139,6 +139,143 @@ int pccl_hip_set_unroll(int unroll);
  * operands' addresses are; -1 = built-in choice (rotated for operands beyond the Infinity Cache). */
 int pccl_hip_set_rotation(int rotate);
 
+/* ---- norms around a block, fused with the fold of its partial outputs -------- */
+/* What a tensor- or sequence-parallel layer runs right behind its reduce-scatter and right in front of its
+ * all-gather, per row of `width` elements:
+ *   y = in[0] + ... + in[n_in-1]              (left fold in input order, binary32)
+ *   n = post(y)                               (norm behind the block)
+ *   r = residual_scale * x + block_scale * g * n
+ *   h = pre(r)                                (norm in front of the next block)
+ * with y, r and h rounded once, each from the binary32 value; nothing that a rounding left is fed on.
+ *   PCCL_NORM_NONE   norm(v) = v
+ *   PCCL_NORM_RMS    norm(v) = v / sqrt(mean(v^2) + eps) * (weight + weight_offset) + bias
+ *   PCCL_NORM_LAYER  the same of v - mean(v)
+ * where an absent weight (NULL) counts as factor 1 (weight_offset is then not added) and an absent bias as 0.
+ * x is absent (residual == NULL: 0) or given; g is absent (gate == NULL: 1) or row i / gate_rows of the gate.
+ * Statistics are held in binary32; a row whose sum of squares passes the largest binary32 is outside of
+ * what the norms can do.  No counterpart in the reference, which has no model-side code; the fold and the store to
+ * every output are those of multimem_ld_reduce and multimemStore (utils/multimem.h:12-102). */
+enum pccl_norm_kind { PCCL_NORM_NONE = 0, PCCL_NORM_RMS = 1, PCCL_NORM_LAYER = 2 };
+#define PCCL_NORM_MAX_WIDTH 16384
+
+/* One layer's fold and norms.  Strides are in elements, from one row to the next; an output's must be at least `width`
+ * (a single row's is not looked at), an input's may be anything from 0.  Addresses need element alignment only. */
+typedef struct pccl_fold_norm_desc {
+  int dtype;                 /* of the rows: PCCL_F32, PCCL_BF16 or PCCL_F16                                   */
+  int param_dtype;           /* of weights, biases, gate and their gradients: `dtype` or PCCL_F32              */
+  int post_kind, pre_kind;   /* enum pccl_norm_kind                                                            */
+  float post_eps, pre_eps;   /* looked at where there is a norm; at least the smallest normal binary32         */
+  float weight_offset;       /* added to both norms' weights (1 for weights stored around zero)                */
+  float residual_scale, block_scale;
+  int n_in, n_out;           /* partial outputs of the block 1..8; copies of h 0..8                            */
+  int reserved;
+  long rows, width;          /* rows >= 0, width 1..PCCL_NORM_MAX_WIDTH                                        */
+  const void *post_weight, *post_bias, *pre_weight, *pre_bias;   /* width elements each, NULL: absent          */
+  const void *gate;          /* ceil(rows / gate_rows) rows, NULL: absent                                      */
+  long gate_stride, gate_rows;
+  const void *ins[PCCL_MAX_INPUTS];
+  long in_stride;
+  const void *residual;      /* x, NULL: absent                                                                */
+  long residual_stride;
+  void *residual_out;        /* r, NULL: not stored                                                            */
+  long residual_out_stride;
+  void *folded;              /* y, NULL: not stored                                                            */
+  long folded_stride;
+  void *outs[PCCL_MAX_OUTPUTS]; /* h                                                                           */
+  long out_stride;
+} pccl_fold_norm_desc;
+
+/* The forward pass.  One kernel launch on `stream`, which must belong to the current device; returns without
+ * waiting.  An output may be the same buffer as an input (same address, same stride); other overlaps are undefined. */
+int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream);
+
+/* Gradients.  Of the forward's description the backward pass reads the norms, scales, parameters and gate,
+ *   ins / n_in         the block's partial outputs again, or y as the forward stored it (n_in = 1);
+ *   residual_out       r as the forward stored it (with pre_kind PCCL_NORM_NONE it is not read and may be NULL);
+ *   n_out              how many partial gradients of h there are (0: none).
+ * With dh = the left fold of the grad_outs and dr = grad_residual_out + pre'(dh; r):
+ *   grad_residual      residual_scale * dr
+ *   grad_ins           post'(block_scale * g * dr; y), stored to each
+ *   grad_gate          sums of block_scale * dr * n over the rows that share a gate row
+ *   grad_*_weight / grad_*_bias  sums over all rows
+ * Statistics are computed again from y and r.  Sums over rows are held in binary32 and added in a fixed order: the same call
+ * gives the same bits.  Every pointer may be NULL: the gradient is then not computed, or taken as zero. */
+typedef struct pccl_fold_norm_grads {
+  const void *grad_outs[PCCL_MAX_OUTPUTS];
+  long grad_out_stride;
+  const void *grad_residual_out;
+  long grad_residual_out_stride;
+  void *grad_ins[PCCL_MAX_INPUTS];
+  int n_grad_in;             /* 0..8, independent of n_in: the all-gather behind a reduce-scatter's gradient    */
+  int reserved;
+  long grad_in_stride;
+  void *grad_residual;
+  long grad_residual_stride;
+  void *grad_gate;
+  long grad_gate_stride;
+  void *grad_post_weight, *grad_post_bias, *grad_pre_weight, *grad_pre_bias;
+  void *workspace;           /* pccl_hip_fold_norm_workspace bytes, 16-byte aligned; used while the launches run */
+  long workspace_bytes;
+} pccl_fold_norm_grads;
+
+/* Two kernel launches on `stream` (one if no gradient of a parameter is asked for). */
+int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const pccl_fold_norm_grads *g, void *stream);
+
+/* Bytes of workspace that a backward pass over this many rows needs on the current device, whichever gradients it asks for
+ * (gate_rows = 0: no gate). */
+int pccl_hip_fold_norm_workspace(long rows, long width, long gate_rows, long *bytes);
+
+/* ---- a cache in blocks of 32 elements with a shared scale ----------------------- */
+/* Keys and values of a rank, 8 or 4 bits an element, in pages that the copies above move between ranks.  Layout of the codes is
+ * that of the OCP microscaling formats: 32 consecutive elements of a head (the last block of a head may be shorter)
+ * share one byte s, which stands for 2^(s - 127); an element is
+ *   PCCL_CACHE_F8E4M3   OCP E4M3FN           (largest value 448)
+ *   PCCL_CACHE_F8E5M2   OCP E5M2             (57344)
+ *   PCCL_CACHE_I8       k / 64, |k| <= 127   (127/64)
+ *   PCCL_CACHE_F4E2M1   OCP E2M1             (6), two in a byte, the even element in the low half
+ * Scale: the smallest power of two, from 2^-127 to 2^127, with which no element of the block passes the format's largest value
+ * (so none saturates; the microscaling text's own rule, the exponent of the largest element, would let up to a quarter
+ * of the largest element be cut off); a block of zeros has s = 0.  Elements are divided by the scale, which is exact, and rounded
+ * once, to the nearest, ties to even.  A block that holds an infinity or a NaN gets s = 255 and codes 0 and is read back as
+ * NaN whole.  (Values from 127/64 * 2^127 in f32 or bf16, whose scale for I8 would be 2^128, saturate.)
+ * No counterpart in the reference. */
+enum pccl_cache_format { PCCL_CACHE_F8E4M3 = 0, PCCL_CACHE_F8E5M2 = 1, PCCL_CACHE_I8 = 2, PCCL_CACHE_F4E2M1 = 3 };
+#define PCCL_CACHE_MAX_TENSORS 8
+#define PCCL_CACHE_BLOCK 32
+
+/* n_tensors caches of one shape (keys and values, or those of several layers).  Codes of page p, token t of the page and head
+ * h start at codes + p * code_page + t * code_token + h * code_head (bytes, ceil(head_dim * bits / 8) of them), its scales at
+ * scales + p * scale_page + t * scale_token + h * scale_head (ceil(head_dim / 32) bytes).  Any order of the three that keeps
+ * heads apart; any alignment. */
+typedef struct pccl_cache_desc {
+  int format;                /* enum pccl_cache_format              */
+  int n_tensors;             /* 1..8                                */
+  int heads, head_dim;       /* 1..65536 each                       */
+  long page_tokens, n_pages; /* page_tokens 1..2^20; pages * tokens up to 2^31 - 1 */
+  void *codes[PCCL_CACHE_MAX_TENSORS];
+  long code_page, code_token, code_head;
+  void *scales[PCCL_CACHE_MAX_TENSORS];
+  long scale_page, scale_token, scale_head;
+} pccl_cache_desc;
+
+/* Codes `tokens` rows of heads x head_dim elements (f32, bf16 or f16; strides in elements) of every source and writes
+ * row i to slot slots[i] = page * page_tokens + token of the page (device memory, read when the kernel runs).  A row whose slot is
+ * below 0 or beyond the last page is neither read nor written.  Slots of one call must differ; a slot named twice holds
+ * unspecified codes afterwards, all others are as they should be.  One kernel launch on `stream`, which must belong to the
+ * current device; returns without waiting. */
+int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const void *const *srcs, long src_token_stride, long src_head_stride,
+                         const long *slots, long tokens, void *stream);
+
+/* Reads sequences back: token t < lengths[s] of sequence s (at most max_len) comes from page
+ * page_table[s * table_stride + t / page_tokens] and goes to row row_start[s] + t of every output, or to row s * max_len + t
+ * where row_start is NULL; heads x head_dim elements a row (f32, bf16 or f16; strides in elements), code times scale rounded once.
+ * table_stride is the number of entries of a sequence: tokens behind its last page are not read.  page_table, lengths and
+ * row_start are device memory.  A row outside [0, out_rows), a page below 0 or beyond the last and a token behind its sequence's
+ * length: nothing is written there, what stood in the row stays.  Rows of different sequences must differ. */
+int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *const *outs, long out_token_stride, long out_head_stride,
+                        long out_rows, const int *page_table, long table_stride, const int *lengths, const long *row_start,
+                        int n_seq, long max_len, void *stream);
+
 /* ---- the op-batching path: a DAG of ops drained by one persistent kernel -- */
 
 /* One IR operation as the host hands it over: the C++ payload level of

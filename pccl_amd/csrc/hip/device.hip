@@ -72,6 +72,16 @@ int executor_id() { return g_executor_id.load(std::memory_order_relaxed); }
 static std::atomic<long> g_slice_bytes{32l << 30};
 long slice_bytes() { return g_slice_bytes.load(std::memory_order_relaxed); }
 
+int check_stream(void *stream) {
+  if (!stream) return PCCL_OK;
+  hipDevice_t of = 0;
+  int current = 0;
+  PCCL_HIP_CHECK(hipGetDevice(&current));
+  PCCL_HIP_CHECK(hipStreamGetDevice((hipStream_t)stream, &of));
+  if ((int)of != current) return fail(PCCL_ERR_INVALID_ARG, "the stream belongs to device %d, the current device is %d", (int)of, current);
+  return PCCL_OK;
+}
+
 // ---- the allocator's bookkeeping -----------------------------------------------------
 // One hipMalloc per allocation, the size rounded up to 2 MiB, and a pointer-keyed map of what is
 // live under one mutex: what the reference's allocator specifies (cuda_executor/device.cc:50-51,

@@ -1,0 +1,6 @@
+// fold_norm_inst_f16_f32.hip -- instantiates the norms around a block for f16 rows, f32 parameters.
+#include "fold_norm_kernel.h"
+
+namespace pccl_dev {
+PCCL_DEFINE_FOLD_NORM(PCCL_F16, true)
+}  // namespace pccl_dev

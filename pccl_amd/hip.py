@@ -26,6 +26,15 @@ MAX_INPUTS = 8
 MAX_OUTPUTS = 8
 
 
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+NORMS = {"none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAYER}
+NORM_MAX_WIDTH = 16384
+CACHE_F8E4M3, CACHE_F8E5M2, CACHE_I8, CACHE_F4E2M1 = 0, 1, 2, 3
+CACHE_FORMATS = {"f8e4m3": CACHE_F8E4M3, "f8e5m2": CACHE_F8E5M2, "i8": CACHE_I8, "f4e2m1": CACHE_F4E2M1}
+CACHE_MAX_TENSORS = 8
+CACHE_BLOCK = 32
+
+
 class PcclError(RuntimeError):
     def __init__(self, code, text):
         super().__init__("pccl_hip error %d: %s" % (code, text))
@@ -51,6 +60,51 @@ class OpDesc(ctypes.Structure):
     ]
 
 
+class FoldNormDesc(ctypes.Structure):
+    """struct pccl_fold_norm_desc"""
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("param_dtype", ctypes.c_int), ("post_kind", ctypes.c_int), ("pre_kind", ctypes.c_int),
+        ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+        ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float),
+        ("n_in", ctypes.c_int), ("n_out", ctypes.c_int), ("reserved", ctypes.c_int),
+        ("rows", ctypes.c_long), ("width", ctypes.c_long),
+        ("post_weight", ctypes.c_void_p), ("post_bias", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p), ("pre_bias", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p), ("gate_stride", ctypes.c_long), ("gate_rows", ctypes.c_long),
+        ("ins", ctypes.c_void_p * MAX_INPUTS), ("in_stride", ctypes.c_long),
+        ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_long),
+        ("residual_out", ctypes.c_void_p), ("residual_out_stride", ctypes.c_long),
+        ("folded", ctypes.c_void_p), ("folded_stride", ctypes.c_long),
+        ("outs", ctypes.c_void_p * MAX_OUTPUTS), ("out_stride", ctypes.c_long),
+    ]
+
+
+class FoldNormGrads(ctypes.Structure):
+    """struct pccl_fold_norm_grads"""
+    _fields_ = [
+        ("grad_outs", ctypes.c_void_p * MAX_OUTPUTS), ("grad_out_stride", ctypes.c_long),
+        ("grad_residual_out", ctypes.c_void_p), ("grad_residual_out_stride", ctypes.c_long),
+        ("grad_ins", ctypes.c_void_p * MAX_INPUTS), ("n_grad_in", ctypes.c_int), ("reserved", ctypes.c_int),
+        ("grad_in_stride", ctypes.c_long),
+        ("grad_residual", ctypes.c_void_p), ("grad_residual_stride", ctypes.c_long),
+        ("grad_gate", ctypes.c_void_p), ("grad_gate_stride", ctypes.c_long),
+        ("grad_post_weight", ctypes.c_void_p), ("grad_post_bias", ctypes.c_void_p),
+        ("grad_pre_weight", ctypes.c_void_p), ("grad_pre_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_long),
+    ]
+
+
+class CacheDesc(ctypes.Structure):
+    """struct pccl_cache_desc"""
+    _fields_ = [
+        ("format", ctypes.c_int), ("n_tensors", ctypes.c_int), ("heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("page_tokens", ctypes.c_long), ("n_pages", ctypes.c_long),
+        ("codes", ctypes.c_void_p * CACHE_MAX_TENSORS),
+        ("code_page", ctypes.c_long), ("code_token", ctypes.c_long), ("code_head", ctypes.c_long),
+        ("scales", ctypes.c_void_p * CACHE_MAX_TENSORS),
+        ("scale_page", ctypes.c_long), ("scale_token", ctypes.c_long), ("scale_head", ctypes.c_long),
+    ]
+
+
 _lib = None
 
 
@@ -71,6 +125,11 @@ def lib():
         L.pccl_hip_free.argtypes = [vp]
         L.pccl_hip_reduce_copy.argtypes = [ci, ci, ctypes.POINTER(vp), ci, ctypes.POINTER(vp), ci, cl, vp]
         L.pccl_hip_accumulate.argtypes = [ci, ci, vp, ctypes.POINTER(vp), ci, cl, vp]
+        L.pccl_hip_fold_norm.argtypes = [ctypes.POINTER(FoldNormDesc), vp]
+        L.pccl_hip_fold_norm_backward.argtypes = [ctypes.POINTER(FoldNormDesc), ctypes.POINTER(FoldNormGrads), vp]
+        L.pccl_hip_fold_norm_workspace.argtypes = [cl, cl, cl, ctypes.POINTER(cl)]
+        L.pccl_hip_cache_write.argtypes = [ctypes.POINTER(CacheDesc), ci, ctypes.POINTER(vp), cl, cl, vp, cl, vp]
+        L.pccl_hip_cache_read.argtypes = [ctypes.POINTER(CacheDesc), ci, ctypes.POINTER(vp), cl, cl, cl, vp, cl, vp, vp, ci, cl, vp]
         L.pccl_hip_set_tuning.argtypes = [ci, ci]
         L.pccl_hip_set_occupancy_lds.argtypes = [ci]
         L.pccl_hip_set_unroll.argtypes = [ci]
@@ -182,6 +241,168 @@ def accumulate(dtype, compute, src, outs, count, stream=None):
     a_out = (ctypes.c_void_p * max(len(outs), 1))(*[_addr(x) for x in outs])
     _check(lib().pccl_hip_accumulate(_code(DTYPES, dtype), _code(COMPUTES, compute), ctypes.c_void_p(_addr(src)), a_out,
                                      len(outs), count, ctypes.c_void_p(_addr(stream))))
+
+
+def _many(x, most, what):
+    """A list of operands, its length checked in front of the fixed array that it goes to."""
+    if len(x) > most:
+        raise PcclError(ERR_INVALID_ARG, "%d %s, at most %d" % (len(x), what, most))
+    return [_addr(t) for t in x]
+
+
+def _index(x, itemsize, count, what):
+    """Address of a device array of whole numbers; of one that can tell its size (a torch tensor), the size is checked."""
+    if x is not None and hasattr(x, "element_size") and (x.element_size() != itemsize or x.numel() < count):
+        raise PcclError(ERR_INVALID_ARG, "%s: %d entries of %d bytes, %d of %d are needed" % (what, x.numel(), x.element_size(), count, itemsize))
+    return _addr(x)
+
+
+class FoldNorm:
+    """The norms around a block, fused with the fold of its partial outputs, its gate and its residual scale
+    (pccl_hip_fold_norm); `width` elements a row:
+
+        y = fold(ins)   n = post(y)   r = residual_scale * residual + block_scale * gate * n   h = pre(r)
+
+    post, pre: "none", "rms" or "layer"; weights and biases are device vectors of `param_dtype` (by default the
+    rows' dtype) and may be None; `weight_offset` is added to the weights.  The object holds these settings and
+    a reference to each parameter, nothing of a call: it may be used from several threads at once."""
+
+    def __init__(self, dtype, width, post="none", pre="rms", param_dtype=None, post_weight=None, post_bias=None, pre_weight=None,
+                 pre_bias=None, post_eps=1e-6, pre_eps=1e-6, weight_offset=0.0, residual_scale=1.0, block_scale=1.0):
+        self._keep = (post_weight, post_bias, pre_weight, pre_bias)
+        self.width = width
+        d = self._desc = FoldNormDesc()
+        d.dtype = _code(DTYPES, dtype)
+        d.param_dtype = d.dtype if param_dtype is None else _code(DTYPES, param_dtype)
+        d.post_kind, d.pre_kind = _code(NORMS, post), _code(NORMS, pre)
+        d.post_eps, d.pre_eps, d.weight_offset = post_eps, pre_eps, weight_offset
+        d.residual_scale, d.block_scale = residual_scale, block_scale
+        d.width = width
+        d.post_weight, d.post_bias, d.pre_weight, d.pre_bias = (_addr(x) for x in self._keep)
+
+    def _call(self, ins, rows, gate, gate_rows, gate_stride, in_stride):
+        d = FoldNormDesc.from_buffer_copy(self._desc)
+        at = _many(ins, MAX_INPUTS, "inputs")
+        d.ins[:len(at)] = at
+        d.n_in, d.rows = len(at), rows
+        d.in_stride = self.width if in_stride is None else in_stride
+        if gate is not None:
+            d.gate, d.gate_rows = _addr(gate), gate_rows
+            d.gate_stride = self.width if gate_stride is None else gate_stride
+        return d
+
+    def forward(self, ins, outs, rows, residual=None, residual_out=None, folded=None, gate=None, gate_rows=0, stream=None,
+                in_stride=None, residual_stride=None, residual_out_stride=None, folded_stride=None, gate_stride=None, out_stride=None):
+        """h to every buffer of `outs` (none: h is not computed), r to `residual_out`, y to `folded`, where given.  The gate
+        has one row for every `gate_rows` rows.  Strides in elements from row to row, by default the width."""
+        w = self.width
+        d = self._call(ins, rows, gate, gate_rows, gate_stride, in_stride)
+        at = _many(outs, MAX_OUTPUTS, "outputs")
+        d.outs[:len(at)] = at
+        d.n_out, d.out_stride = len(at), w if out_stride is None else out_stride
+        d.residual, d.residual_stride = _addr(residual), w if residual_stride is None else residual_stride
+        d.residual_out, d.residual_out_stride = _addr(residual_out), w if residual_out_stride is None else residual_out_stride
+        d.folded, d.folded_stride = _addr(folded), w if folded_stride is None else folded_stride
+        _check(lib().pccl_hip_fold_norm(ctypes.byref(d), _addr(stream)))
+
+    def workspace_bytes(self, rows, gate_rows=0):
+        """Bytes of workspace that backward needs for this many rows (gate_rows = 0: no gate)."""
+        n = ctypes.c_long(0)
+        _check(lib().pccl_hip_fold_norm_workspace(rows, self.width, gate_rows, ctypes.byref(n)))
+        return n.value
+
+    def backward(self, ins, grad_outs, grad_ins, rows, residual_out=None, grad_residual_out=None, grad_residual=None, gate=None,
+                 gate_rows=0, grad_gate=None, grad_post_weight=None, grad_post_bias=None, grad_pre_weight=None, grad_pre_bias=None,
+                 workspace=None, workspace_bytes=None, stream=None, in_stride=None, residual_out_stride=None, gate_stride=None,
+                 grad_out_stride=None, grad_residual_out_stride=None, grad_in_stride=None, grad_residual_stride=None, grad_gate_stride=None):
+        """Gradients (pccl_hip_fold_norm_backward).  ins: the block's partial outputs again, or [folded]; residual_out: r of
+        the forward pass; grad_outs: the partial gradients of h, folded here; grad_residual_out: the gradient of r from
+        further on.  Written where given: grad_ins (each the gradient of y), grad_residual, grad_gate and those of the
+        parameters.  workspace: a buffer of workspace_bytes(rows, gate_rows), its size taken from the buffer where it can
+        tell (a torch tensor), else from the argument."""
+        w = self.width
+        d = self._call(ins, rows, gate, gate_rows, gate_stride, in_stride)
+        d.residual_out, d.residual_out_stride = _addr(residual_out), w if residual_out_stride is None else residual_out_stride
+        g = FoldNormGrads()
+        at = _many(grad_outs, MAX_OUTPUTS, "gradients of the outputs")
+        g.grad_outs[:len(at)] = at
+        d.n_out, g.grad_out_stride = len(at), w if grad_out_stride is None else grad_out_stride
+        at = _many(grad_ins, MAX_INPUTS, "gradients of the inputs")
+        g.grad_ins[:len(at)] = at
+        g.n_grad_in, g.grad_in_stride = len(at), w if grad_in_stride is None else grad_in_stride
+        g.grad_residual_out = _addr(grad_residual_out)
+        g.grad_residual_out_stride = w if grad_residual_out_stride is None else grad_residual_out_stride
+        g.grad_residual, g.grad_residual_stride = _addr(grad_residual), w if grad_residual_stride is None else grad_residual_stride
+        g.grad_gate, g.grad_gate_stride = _addr(grad_gate), w if grad_gate_stride is None else grad_gate_stride
+        g.grad_post_weight, g.grad_post_bias = _addr(grad_post_weight), _addr(grad_post_bias)
+        g.grad_pre_weight, g.grad_pre_bias = _addr(grad_pre_weight), _addr(grad_pre_bias)
+        if workspace is not None:
+            if workspace_bytes is None:
+                workspace_bytes = workspace.numel() * workspace.element_size()
+            g.workspace, g.workspace_bytes = _addr(workspace), workspace_bytes
+        _check(lib().pccl_hip_fold_norm_backward(ctypes.byref(d), ctypes.byref(g), _addr(stream)))
+
+
+class Cache:
+    """A cache of keys and values in pages, coded in blocks of 32 elements with a shared power-of-two scale
+    (pccl_cache_desc): codes and scales are one device buffer per tensor (keys, values, ...).  The layout is pages x tokens of a
+    page x heads x bytes of a head unless strides in bytes, (page, token, head), say otherwise."""
+
+    def __init__(self, fmt, heads, head_dim, page_tokens, n_pages, codes, scales, code_strides=None, scale_strides=None):
+        self._keep = (list(codes), list(scales))
+        self.heads, self.head_dim, self.page_tokens, self.n_pages = heads, head_dim, page_tokens, n_pages
+        d = self._desc = CacheDesc()
+        d.format = _code(CACHE_FORMATS, fmt)
+        d.heads, d.head_dim, d.page_tokens, d.n_pages = heads, head_dim, page_tokens, n_pages
+        codes, scales = _many(codes, CACHE_MAX_TENSORS, "tensors of codes"), _many(scales, CACHE_MAX_TENSORS, "tensors of scales")
+        if len(codes) != len(scales):
+            raise PcclError(ERR_INVALID_ARG, "%d tensors of codes, %d of scales" % (len(codes), len(scales)))
+        d.n_tensors = self.n_tensors = len(codes)
+        d.codes[:len(codes)], d.scales[:len(scales)] = codes, scales
+        row, blocks = self.row_bytes(fmt, head_dim)
+        d.code_page, d.code_token, d.code_head = code_strides or (page_tokens * heads * row, heads * row, row)
+        d.scale_page, d.scale_token, d.scale_head = scale_strides or (page_tokens * heads * blocks, heads * blocks, blocks)
+
+    @staticmethod
+    def row_bytes(fmt, head_dim):
+        """(bytes of codes, bytes of scales) of one token's head"""
+        bits = 4 if _code(CACHE_FORMATS, fmt) == CACHE_F4E2M1 else 8
+        return (head_dim * bits + 7) // 8, (head_dim + CACHE_BLOCK - 1) // CACHE_BLOCK
+
+    def _operands(self, x, what):
+        if len(x) != self.n_tensors:
+            raise PcclError(ERR_INVALID_ARG, "%d %s for %d tensors" % (len(x), what, self.n_tensors))
+        return (ctypes.c_void_p * len(x))(*[_addr(t) for t in x])
+
+    def write(self, dtype, srcs, slots, tokens, stream=None, token_stride=None, head_stride=None):
+        """Codes `tokens` rows of heads x head_dim elements of every source into slots[i] = page * page_tokens + token of the page
+        (int64 on the device; a slot outside the cache: the row is left out).  The slots of one call must differ.  Strides in
+        elements, by default those of a dense [tokens, heads, head_dim]."""
+        srcs = self._operands(srcs, "sources")
+        head_stride = self.head_dim if head_stride is None else head_stride
+        token_stride = self.heads * self.head_dim if token_stride is None else token_stride
+        _check(lib().pccl_hip_cache_write(ctypes.byref(self._desc), _code(DTYPES, dtype), srcs, token_stride, head_stride,
+                                          _index(slots, 8, tokens, "slots"), tokens, _addr(stream)))
+
+    def read(self, dtype, outs, page_table, lengths, n_seq, max_len, row_start=None, out_rows=None, table_stride=None, stream=None,
+             token_stride=None, head_stride=None):
+        """Token t < lengths[s] of sequence s, from page page_table[s][t // page_tokens], to row row_start[s] + t of every output (of
+        `out_rows` rows), or without row_start to row s * max_len + t.  page_table, lengths (int32) and row_start (int64) are on
+        the device; table_stride, the entries of a sequence, is by default what a dense 2-d table says.  Rows that no token goes to
+        are left as they are."""
+        outs = self._operands(outs, "outputs")
+        head_stride = self.head_dim if head_stride is None else head_stride
+        token_stride = self.heads * self.head_dim if token_stride is None else token_stride
+        if table_stride is None:
+            table_stride = page_table.shape[-1]
+        if out_rows is None:
+            if row_start is not None:
+                raise PcclError(ERR_INVALID_ARG, "row_start without out_rows")
+            out_rows = n_seq * max_len
+        _check(lib().pccl_hip_cache_read(ctypes.byref(self._desc), _code(DTYPES, dtype), outs, token_stride, head_stride, out_rows,
+                                         _index(page_table, 4, n_seq * table_stride, "page_table"), table_stride,
+                                         _index(lengths, 4, n_seq, "lengths"), _index(row_start, 8, n_seq, "row_start"), n_seq, max_len,
+                                         _addr(stream)))
 
 
 def _op_descs(ops):
