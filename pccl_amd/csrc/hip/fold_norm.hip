@@ -15,14 +15,14 @@ namespace {
 // Rows of a launch: a grid times its lanes must fit 32 bits, 2^22 - 1 workgroups of 1024.
 constexpr unsigned kLaunchRows = 1u << 21;
 
-// Teams of the smallest shape that holds the width: a wavefront up to 1024 elements (no barrier in its sums), a
+// Teams of the smallest shape that holds the width: a wavefront up to 512 elements (no barrier in its sums), a
 // workgroup beyond.
 NormShape shape_of(long width) {
   if (width <= 512) return {64, 8};
-  if (width <= 1024) return {64, 16};
+  if (width <= 1024) return {128, 8};
   if (width <= 2048) return {256, 8};
-  if (width <= 4096) return {256, 16};
-  if (width <= 8192) return {512, 16};
+  if (width <= 4096) return {512, 8};
+  if (width <= 8192) return {1024, 8};
   return {1024, 16};
 }
 
@@ -136,7 +136,7 @@ struct Cut {
 // (4 rows of binary32 a team) stays small beside the rows themselves.
 Cut cut_of(long rows, long width, long gate_rows) {
   const NormShape n = shape_of(width);
-  const long most = (long)pccl_host::compute_units() * (n.lanes == 64 ? 16 : std::max(1, 2048 / n.lanes / 2));
+  const long most = (long)pccl_host::compute_units() * (1024 / n.lanes);
   const long per = gate_rows >= 1 ? std::min(gate_rows, std::max(1l, rows)) : std::max(1l, rows);
   Cut c;
   c.groups = (unsigned)std::max(1l, gate_row_count(rows, per));
@@ -271,9 +271,9 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   a.grad_gate = d->rows ? (char *)g->grad_gate : nullptr;  // (no rows: no gate row either)
   a.grad_gate_bytes = g->grad_gate_stride * c.ps;
   for (int k = 0; k < 4; ++k) a.want_sums[k] = to[k] != nullptr;
-  const bool full = g->grad_gate || to[1] || to[3];
+  const bool bias = to[1] || to[3] || (g->grad_gate && d->post_bias);
   rc = launched(with_types(d->dtype, d->param_dtype, [&](auto t, auto p) {
-    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape_of(d->width), full, (hipStream_t)stream, a);
+    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape_of(d->width), bias, (hipStream_t)stream, a);
   }), "fold_norm_backward");
   if (rc != PCCL_OK || !need) return rc;
 

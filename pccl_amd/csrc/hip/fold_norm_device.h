@@ -142,14 +142,17 @@ struct Share {
       }
     }
   }
-  // x = 0 in the elements that are not this lane's
+  // x = 0 in the elements that are not this lane's; wavefronts whose packs are all whole step over it
   __device__ __forceinline__ void mask(float (&x)[E]) const {
     if (ragged) {
 #pragma unroll
-      for (int j = 0; j < kPacks; ++j)
+      for (int j = 0; j < kPacks; ++j) {
+        if (lo[j] != 0) {
 #pragma unroll
-        for (int i = 0; i < R::kPack; ++i)
-          if (i < lo[j]) x[j * R::kPack + i] = 0.0f;
+          for (int i = 0; i < R::kPack; ++i)
+            if (i < lo[j]) x[j * R::kPack + i] = 0.0f;
+        }
+      }
     }
   }
   static __device__ __forceinline__ void up(const u32x4 (&v)[kPacks], float (&x)[E]) {
@@ -202,8 +205,8 @@ struct ParamShare {
 };
 
 // y = the left fold of this lane's share of n rows.  AT_ONCE inputs are in flight together.
-template <class R, int LANES, int E, int AT_ONCE>
-__device__ __forceinline__ void fold_rows(const Share<R, LANES, E> &s, const char *const *ins, int n, long at, float (&y)[E]) {
+template <class R, int LANES, int E, int AT_ONCE, class Ins>
+__device__ __forceinline__ void fold_rows(const Share<R, LANES, E> &s, const Ins &ins, int n, long at, float (&y)[E]) {
   constexpr int kPacks = E / R::kPack;
   for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
     u32x4 v[AT_ONCE][kPacks];
@@ -227,51 +230,57 @@ __device__ __forceinline__ void fold_rows(const Share<R, LANES, E> &s, const cha
   }
 }
 
-// Lane 63's value after a sum over the wavefront by shifts inside rows of 16 lanes and broadcasts of
-// each row's last lane: six vector adds and no LDS access.  All 64 lanes are active.
+// Sums over lanes by data-parallel-primitive adds, no LDS access: shifts inside rows of 16 lanes leave a row's sum in its last
+// lane, broadcasts of those the wavefront's sum in lane 63.  All 64 lanes are active.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float plus_dpp(float x) {
   return x + as_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)as_u32(x), CTRL, ROWS, 0xf, false));
 }
-__device__ __forceinline__ float wave_sum(float x) {
+__device__ __forceinline__ float row_sum(float x) {  // in lanes 15, 31, 47, 63
   x = plus_dpp<0x111, 0xf>(x);  // row_shr:1
   x = plus_dpp<0x112, 0xf>(x);  // row_shr:2
   x = plus_dpp<0x114, 0xf>(x);  // row_shr:4
-  x = plus_dpp<0x118, 0xf>(x);  // row_shr:8
-  x = plus_dpp<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
-  x = plus_dpp<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
-  return as_f32((unsigned)__builtin_amdgcn_readlane((int)as_u32(x), 63));
+  return plus_dpp<0x118, 0xf>(x);  // row_shr:8
 }
+__device__ __forceinline__ float wave_sum(float x) {  // in lane 63
+  x = row_sum(x);
+  x = plus_dpp<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  return plus_dpp<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ float of_lane(float x, int lane) { return as_f32((unsigned)__builtin_amdgcn_readlane((int)as_u32(x), lane)); }
 
-// Sums over a team, the same value in every lane, added in the same order every time.  `turn` alternates between
-// two sets of LDS words, so that one barrier a sum is enough: a wavefront writes a set again only
+// Sums over a team, the same value in every lane, added in the same order every time: the wavefronts' sums go to LDS,
+// the sixteen lanes of a row read one each and add them as above (reading all of them into every lane cost 64 registers).
+// `turn` alternates between two sets of LDS words, so that one barrier a sum is enough: a wavefront writes a set again only
 // after the barrier of the sum in between, which every reader of the set has reached.
 constexpr int kSumsAtOnce = 4;
 template <int LANES>
 struct TeamSums {
   static constexpr int kWaves = LANES / kWave;
-  float (*words)[kWaves > 1 ? kWaves : 1][kSumsAtOnce];  // [2]
+  static_assert(kWaves <= 16, "one lane of a row per wavefront");
+  float (*words)[kWaves][kSumsAtOnce];  // [2]
   int turn;
 
   template <int N>
   __device__ __forceinline__ void operator()(float (&x)[N]) {
+    if constexpr (kWaves == 1) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) x[n] = wave_sum(x[n]);
-    if constexpr (kWaves > 1) {
-      const int wave = (int)threadIdx.x / kWave;
+      for (int n = 0; n < N; ++n) x[n] = of_lane(wave_sum(x[n]), kWave - 1);
+    } else {
       float (*w)[kSumsAtOnce] = words[turn];
-      if ((threadIdx.x & (kWave - 1)) == 0) {
+      const int wave = (int)threadIdx.x / kWave, lane = (int)threadIdx.x % kWave;
+#pragma unroll
+      for (int n = 0; n < N; ++n) x[n] = wave_sum(x[n]);
+      if (lane == kWave - 1) {
 #pragma unroll
         for (int n = 0; n < N; ++n) w[wave][n] = x[n];
       }
       __syncthreads();
+      const int from = lane % 16;
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        float t = w[0][n];
+      for (int n = 0; n < N; ++n) x[n] = from < kWaves ? w[from < kWaves ? from : 0][n] : 0.0f;
 #pragma unroll
-        for (int k = 1; k < kWaves; ++k) t += w[k][n];
-        x[n] = t;
-      }
+      for (int n = 0; n < N; ++n) x[n] = of_lane(row_sum(x[n]), 15);
       turn ^= 1;
     }
   }

@@ -72,7 +72,8 @@ __device__ __forceinline__ void scale_and_shift(const Share<R, LANES, E> &s, con
   }
 }
 
-constexpr int team_block(int lanes) { return lanes < kBlock ? kBlock : lanes; }
+// Lanes of a workgroup: teams of one wavefront come four to a workgroup (they meet at no barrier), others have their own.
+constexpr int team_block(int lanes) { return lanes == kWave ? kBlock : lanes; }
 
 template <int DT, bool PF32, int LANES, int E, int AT_ONCE>
 __global__ void __launch_bounds__(team_block(LANES)) fold_norm_kernel(const ForwardArgs a) {
@@ -165,96 +166,163 @@ __device__ __forceinline__ void store_sums(const Share<R, LANES, E> &s, float *r
   }
 }
 
-// FULL: sums for biases and gate as well (registers for five rows of sums instead of two)
-template <int DT, bool PF32, int LANES, int E, bool FULL>
-__global__ void __launch_bounds__(team_block(LANES)) fold_norm_backward_kernel(const BackwardArgs a) {
+// x = the lane's share of a row of sums, or zeros
+template <class R, int LANES, int E>
+__device__ __forceinline__ void load_sums(const Share<R, LANES, E> &s, const float *row, bool there, float (&x)[E]) {
+#pragma unroll
+  for (int j = 0; j < E / R::kPack; ++j)
+#pragma unroll
+    for (int i = 0; i < R::kPack; ++i) x[j * R::kPack + i] = there && i >= s.lo[j] ? row[s.off[j] + i] : 0.0f;
+}
+
+// What a row of the backward pass sums over the team: a parameter's column sums come from two products per element.
+// With yhat, rhat the standardised y and r:
+//   s1 = sum dr * yhat, s0 = sum dr over the rows of a strip, which share a gate row g, give
+//     the gate's gradient            c * ((w + o) * s1 + b * s0)        (c block_scale, w, o, b the post norm's)
+//     the post norm's                weight c * g * s1, bias c * g * s0
+//   p1 = sum dh * rhat, p0 = sum dh  weight and bias of the pre norm
+// so that a row costs one fused multiply-add a column for each, and gate and weight are met once a strip.
+//
+// One team's registers hold the row (packed), the row after it on its way (SINGLE: one y and at most one dh, so that
+// four streams are read), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, and the sums.
+// BIAS: some bias's gradient or a gate behind a biased norm is asked for (s0 and p0 are kept).
+//
+// The arguments (18 addresses and 12 strides) are read again from the argument segment wherever a row needs them: held
+// in scalar registers over the loop they spill into vector registers, and those are what is short here.
+typedef const BackwardArgs __attribute__((address_space(4))) *BackwardArgsAt;
+__device__ __forceinline__ BackwardArgsAt read_again(BackwardArgsAt p) {
+  asm volatile("" : "+s"(p));  // (no instruction: the compiler may not know what it points to any more)
+  return p;
+}
+template <class R, int LANES, int E>
+struct BackRow {
+  u32x4 y[E / R::kPack], r[E / R::kPack], dh[E / R::kPack], dr[E / R::kPack];
+};
+
+template <int DT, bool PF32, int LANES, int E, bool SINGLE, bool BIAS>
+__global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kernel(const BackwardArgs) {
   typedef RowType<DT> R;
   typedef Share<R, LANES, E> S;
   typedef ParamShare<R, PF32, LANES, E> P;
-  constexpr int kPacks = E / R::kPack;
   constexpr int kTeams = team_block(LANES) / LANES;
   constexpr int kFold = 4;  // gradients in flight together; more cost registers
+  const BackwardArgsAt args = (BackwardArgsAt)__builtin_amdgcn_kernarg_segment_ptr();  // (the one argument stands at its start)
+  const BackwardArgsAt a0 = args;
   __shared__ float words[2][LANES / kWave][kSumsAtOnce];
   const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / LANES);
   const unsigned t = blockIdx.x * kTeams + team;
-  if (t >= a.n_teams) return;
-  const S s((int)threadIdx.x % LANES, a.width);
+  if (t >= a0->n_teams) return;
+  const S s((int)threadIdx.x % LANES, a0->width);
   TeamSums<LANES> sums{words, 0};
-  const bool post = a.post_kind != PCCL_NORM_NONE, pre = a.pre_kind != PCCL_NORM_NONE;
-  const bool post_layer = a.post_kind == PCCL_NORM_LAYER, pre_layer = a.pre_kind == PCCL_NORM_LAYER;
+  const bool post = a0->post_kind != PCCL_NORM_NONE, outs = a0->n_out > 0, pre = a0->pre_kind != PCCL_NORM_NONE && outs;
+  const bool post_layer = a0->post_kind == PCCL_NORM_LAYER, pre_layer = pre && a0->pre_kind == PCCL_NORM_LAYER;
+  const float per_width = a0->per_width;
 
-  float sum_post[E], sum_pre[E], sum_post_bias[FULL ? E : 1], sum_pre_bias[FULL ? E : 1], sum_gate[FULL ? E : 1];
+  float wpre[E], p1[E], p0[BIAS ? E : 1];
 #pragma unroll
-  for (int i = 0; i < E; ++i) sum_post[i] = sum_pre[i] = 0.0f;
-  if constexpr (FULL) {
+  for (int i = 0; i < E; ++i) {
+    wpre[i] = 1.0f;
+    p1[i] = 0.0f;
+    if constexpr (BIAS) p0[i] = 0.0f;
+  }
+  if (a0->pre_weight) {
+    P w;
+    w.load(s, a0->pre_weight);
+    w.up(wpre);
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum_post_bias[i] = sum_pre_bias[i] = 0.0f;
+    for (int i = 0; i < E; ++i) wpre[i] += a0->weight_offset;
   }
 
-  const unsigned first = (unsigned)((unsigned long)a.n_strips * t / a.n_teams);
-  const unsigned end = (unsigned)((unsigned long)a.n_strips * (t + 1) / a.n_teams);
-  for (unsigned strip = first; strip < end; ++strip) {
-    const unsigned group = strip / a.strips;
-    // (the last gate row may have fewer rows than gate_rows, and its last strips then none: 64 bits, and no row)
-    const unsigned long group_row = (unsigned long)group * a.gate_rows;
-    const unsigned long begin = group_row + (unsigned long)(strip - group * a.strips) * a.strip_rows;
-    unsigned long stop = begin + a.strip_rows;
-    if (stop > group_row + a.gate_rows) stop = group_row + a.gate_rows;
-    if (stop > a.rows) stop = a.rows;
-    const char *gate_row = a.gate ? a.gate + group * a.gate_bytes : nullptr;
-    if constexpr (FULL) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) sum_gate[i] = 0.0f;
+  auto load_row = [&](unsigned long row, BackRow<R, LANES, E> &x) {
+    const BackwardArgsAt a = read_again(args);
+    if (a->grad_residual_out) s.load(a->grad_residual_out + row * a->grad_residual_out_bytes, x.dr);
+    if (pre) s.load(a->residual_out + row * a->residual_out_bytes, x.r);
+    if constexpr (SINGLE) {
+      if (outs) s.load(a->grad_outs[0] + row * a->grad_out_bytes, x.dh);
+      s.load(a->ins[0] + row * a->in_bytes, x.y);
     }
-    for (unsigned long row = begin; row < stop; ++row) {
-      u32x4 v_r[kPacks], v_dr[kPacks];
-      float y[E], dh[E], dr[E];
-      P w_pre, w_post, gate;
-      if (a.grad_residual_out) s.load(a.grad_residual_out + row * a.grad_residual_out_bytes, v_dr);
-      if (pre && a.n_out) s.load(a.residual_out + (long)row * a.residual_out_bytes, v_r);
-      if (a.n_out) fold_rows<R, LANES, E, kFold>(s, a.grad_outs, a.n_out, row * a.grad_out_bytes, dh);
-      fold_rows<R, LANES, E, kFold>(s, a.ins, a.n_in, (long)row * a.in_bytes, y);
-      if (a.pre_weight) w_pre.load(s, a.pre_weight);
-      if (a.post_weight) w_post.load(s, a.post_weight);
-      if (gate_row) gate.load(s, gate_row);
-      if (a.grad_residual_out) {
-        s.up(v_dr, dr);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] = 0.0f;
-      }
+  };
 
+  const unsigned first = (unsigned)((unsigned long)a0->n_strips * t / a0->n_teams);
+  const unsigned end = (unsigned)((unsigned long)a0->n_strips * (t + 1) / a0->n_teams);
+  for (unsigned strip = first; strip < end; ++strip) {
+    const BackwardArgsAt a1 = read_again(args);
+    const unsigned group = strip / a1->strips;
+    // (the last gate row may have fewer rows than gate_rows, and its last strips then none: 64 bits, and no row)
+    const unsigned long group_row = (unsigned long)group * a1->gate_rows;
+    const unsigned long begin = group_row + (unsigned long)(strip - group * a1->strips) * a1->strip_rows;
+    unsigned long stop = begin + a1->strip_rows;
+    if (stop > group_row + a1->gate_rows) stop = group_row + a1->gate_rows;
+    if (stop > a1->rows) stop = a1->rows;
+
+    BackRow<R, LANES, E> next;
+    if (SINGLE && begin < stop) load_row(begin, next);
+    float cgw[E], s1[E], s0[BIAS ? E : 1];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      cgw[i] = a1->block_scale;
+      s1[i] = 0.0f;
+      if constexpr (BIAS) s0[i] = 0.0f;
+    }
+    if (a1->gate) {
+      P g;
+      float f[E];
+      g.load(s, a1->gate + group * a1->gate_bytes);
+      g.up(f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) cgw[i] *= f[i];
+    }
+    if (a1->post_weight) {
+      P w;
+      float f[E];
+      w.load(s, a1->post_weight);
+      w.up(f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) cgw[i] *= f[i] + a1->weight_offset;
+    }
+
+    for (unsigned long row = begin; row < stop; ++row) {
+      BackRow<R, LANES, E> now;
+      float y[E], dh[E], r[E];
+      if constexpr (SINGLE) {
+        now = next;
+        if (row + 1 < stop) load_row(row + 1, next);
+        s.up(now.y, y);
+        if (outs) s.up(now.dh, dh);
+      } else {
+        load_row(row, now);
+        const BackwardArgsAt a = read_again(args);
+        if (outs) fold_rows<R, LANES, E, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh);
+        fold_rows<R, LANES, E, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y);
+      }
       s.mask(y);
-      s.mask(dr);
-      if (a.n_out) s.mask(dh);
-      // both norms' statistics, and what the pre norm's backward sums, in one go over the team (two with a layer norm)
-      float r[E], mean_y = 0.0f;
-      const bool through_pre = pre && a.n_out;
-      if (through_pre) {
-        s.up(v_r, r);
+      if (outs) s.mask(dh);
+      if (pre) {
+        s.up(now.r, r);
         s.mask(r);
       }
-      if ((post && post_layer) || (through_pre && pre_layer)) {
+      // both norms' statistics, and what the pre norm's backward sums, in one go over the team (two with a layer norm)
+      if (post_layer || pre_layer) {
         float m[2] = {0.0f, 0.0f};
-        if (post && post_layer) {
+        if (post_layer) {
 #pragma unroll
           for (int i = 0; i < E; ++i) m[0] += y[i];
         }
-        if (through_pre && pre_layer) {
+        if (pre_layer) {
 #pragma unroll
           for (int i = 0; i < E; ++i) m[1] += r[i];
         }
         sums(m);
-        if (post && post_layer) {
-          mean_y = m[0] * a.per_width;
+        if (post_layer) {
+          const float mean = m[0] * per_width;
 #pragma unroll
-          for (int i = 0; i < E; ++i) y[i] -= mean_y;
+          for (int i = 0; i < E; ++i) y[i] -= mean;
           s.mask(y);
         }
-        if (through_pre && pre_layer) {
-          const float mean_r = m[1] * a.per_width;
+        if (pre_layer) {
+          const float mean = m[1] * per_width;
 #pragma unroll
-          for (int i = 0; i < E; ++i) r[i] -= mean_r;
+          for (int i = 0; i < E; ++i) r[i] -= mean;
           s.mask(r);
         }
       }
@@ -263,122 +331,159 @@ __global__ void __launch_bounds__(team_block(LANES)) fold_norm_backward_kernel(c
 #pragma unroll
         for (int i = 0; i < E; ++i) q[0] = __builtin_fmaf(y[i], y[i], q[0]);
       }
-      float d[E];  // dh * w
-      if (through_pre) {
-        if (a.pre_weight) {
-          float w[E];
-          w_pre.up(w);
-#pragma unroll
-          for (int i = 0; i < E; ++i) d[i] = dh[i] * (w[i] + a.weight_offset);
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; ++i) d[i] = dh[i];
-        }
+      if (pre) {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           q[1] = __builtin_fmaf(r[i], r[i], q[1]);
-          q[2] = __builtin_fmaf(d[i], r[i], q[2]);
-          q[3] += d[i];
+          q[2] = __builtin_fmaf(dh[i] * wpre[i], r[i], q[2]);
+        }
+        if (pre_layer) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) q[3] = __builtin_fmaf(dh[i], wpre[i], q[3]);
         }
       }
-      if (post || through_pre) sums(q);
-      if (through_pre) {
-        const float rstd = one_over_spread(q[1], a.per_width, a.pre_eps);
-        const float along = q[2] * rstd * a.per_width, mean_d = pre_layer ? q[3] * a.per_width : 0.0f;
+      if (post || pre) sums(q);
+      const BackwardArgsAt a = read_again(args);
+      float dr[E];
+      if (a->grad_residual_out) {
+        s.up(now.dr, dr);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) dr[i] = 0.0f;
+      }
+      if (pre) {
+        // dr += rstd * (d - rhat * mean(d * rhat) - mean(d)), d = dh * w
+        const float rstd = one_over_spread(q[1], per_width, a->pre_eps);
+        const float along = -(rstd * rstd * rstd) * (q[2] * per_width);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const float hat = r[i] * rstd;
-          sum_pre[i] = __builtin_fmaf(dh[i], hat, sum_pre[i]);
-          dr[i] = __builtin_fmaf(rstd, d[i] - __builtin_fmaf(hat, along, mean_d), dr[i]);
+          p1[i] = __builtin_fmaf(dh[i], r[i] * rstd, p1[i]);
+          dr[i] = __builtin_fmaf(dh[i] * wpre[i], rstd, __builtin_fmaf(r[i], along, dr[i]));
         }
-        if constexpr (FULL) {
+        if (pre_layer) {
+          const float mean = rstd * (q[3] * per_width);
 #pragma unroll
-          for (int i = 0; i < E; ++i) sum_pre_bias[i] += dh[i];
+          for (int i = 0; i < E; ++i) dr[i] -= mean;
         }
-        if (pre_layer) s.mask(dr);  // (the mean of d went into masked elements)
-      } else if (a.n_out) {
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) p0[i] += dh[i];
+        }
+      } else if (outs) {
 #pragma unroll
         for (int i = 0; i < E; ++i) dr[i] += dh[i];
       }
-      if (a.grad_residual) {
+      s.mask(dr);
+      if (a->grad_residual) {
         float x[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = a.residual_scale * dr[i];
-        s.store(a.grad_residual + row * a.grad_residual_bytes, x);
+        for (int i = 0; i < E; ++i) x[i] = a->residual_scale * dr[i];
+        s.store(a->grad_residual + row * a->grad_residual_bytes, x);
       }
-#pragma unroll
-      for (int i = 0; i < E; ++i) dr[i] *= a.block_scale;
-      float rstd_y = 1.0f;
       if (post) {
-        rstd_y = one_over_spread(q[0], a.per_width, a.post_eps);
-#pragma unroll
-        for (int i = 0; i < E; ++i) y[i] *= rstd_y;
-      }
-      float w[E];
-      if (a.post_weight) {
-        w_post.up(w);
-#pragma unroll
-        for (int i = 0; i < E; ++i) w[i] += a.weight_offset;
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) w[i] = 1.0f;
-      }
-      if (gate_row) {
-        float g[E];
-        gate.up(g);
-        if constexpr (FULL) {
-          float b[E];
-          if (a.post_bias) {
-            P bias;
-            bias.load(s, a.post_bias);
-            bias.up(b);
-          } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) b[i] = 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < E; ++i) sum_gate[i] = __builtin_fmaf(dr[i], __builtin_fmaf(y[i], w[i], b[i]), sum_gate[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] *= g[i];
-      }
-      if (post) {  // dr is the gradient of n now, y standardised
-        if constexpr (FULL) {
-#pragma unroll
-          for (int i = 0; i < E; ++i) sum_post_bias[i] += dr[i];
-        }
+        const float rstd = one_over_spread(q[0], per_width, a->post_eps);
         float m[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          sum_post[i] = __builtin_fmaf(dr[i], y[i], sum_post[i]);
-          dr[i] *= w[i];
+          y[i] *= rstd;
+          s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
+        }
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) s0[i] += dr[i];
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          dr[i] *= cgw[i];
           m[0] = __builtin_fmaf(dr[i], y[i], m[0]);
-          m[1] += dr[i];
+        }
+        if (post_layer) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) m[1] += dr[i];
         }
         sums(m);
-        const float along = m[0] * a.per_width, mean_d = post_layer ? m[1] * a.per_width : 0.0f;
+        const float along = -rstd * (m[0] * per_width), mean = -rstd * (m[1] * per_width);
 #pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] = rstd_y * (dr[i] - __builtin_fmaf(y[i], along, mean_d));
+        for (int i = 0; i < E; ++i) dr[i] = __builtin_fmaf(dr[i], rstd, __builtin_fmaf(y[i], along, mean));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
+          dr[i] *= cgw[i];
+        }
       }
-      const long at = row * a.grad_in_bytes;
-#pragma unroll
-      for (int j = 0; j < PCCL_MAX_INPUTS; ++j)
-        if (j < a.n_grad_in) s.store(a.grad_ins[j] + at, dr);
+      const unsigned long at = row * a->grad_in_bytes;
+#pragma unroll 1
+      for (int j = 0; j < a->n_grad_in; ++j) s.store(a->grad_ins[j] + at, dr);
     }
-    if constexpr (FULL) {
-      if (a.gate_sums) store_sums(s, a.gate_sums + strip * a.width, sum_gate);
-      else if (a.grad_gate) {
-        if constexpr (PF32 && R::kBytes == 2) store_sums(s, (float *)(a.grad_gate + group * a.grad_gate_bytes), sum_gate);
-        else s.store(a.grad_gate + group * a.grad_gate_bytes, sum_gate);
+
+    // the strip's sums: to the gate's gradient or its workspace, and, times the gate, to the team's
+    const BackwardArgsAt a = read_again(args);
+    if (a->grad_gate) {
+      float x[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = s1[i] * a->block_scale;
+      if (a->post_weight) {
+        P w;
+        float f[E];
+        w.load(s, a->post_weight);
+        w.up(f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] *= f[i] + a->weight_offset;
+      }
+      if constexpr (BIAS) {
+        if (a->post_bias) {
+          P b;
+          float f[E];
+          b.load(s, a->post_bias);
+          b.up(f);
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i] * a->block_scale, s0[i], x[i]);
+        }
+      }
+      if (a->gate_sums) {
+        store_sums(s, a->gate_sums + (unsigned long)strip * a->width, x);
+      } else if constexpr (PF32 && R::kBytes == 2) {
+        store_sums(s, (float *)(a->grad_gate + group * a->grad_gate_bytes), x);
+      } else {
+        s.store(a->grad_gate + group * a->grad_gate_bytes, x);
+      }
+    }
+    if (a->want_sums[0] || a->want_sums[1]) {
+      float f[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = a->block_scale;
+      if (a->gate) {
+        P g;
+        float x[E];
+        g.load(s, a->gate + group * a->gate_bytes);
+        g.up(x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] *= x[i];
+      }
+      // a team of several strips adds to what it wrote itself (each lane to its own columns)
+      float *mine = a->sums + (unsigned long)t * 4 * a->width;
+      float x[E];
+      if (a->want_sums[0]) {
+        load_sums(s, mine, strip != first, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i], s1[i], x[i]);
+        store_sums(s, mine, x);
+      }
+      if constexpr (BIAS) {
+        if (a->want_sums[1]) {
+          load_sums(s, mine + a->width, strip != first, x);
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i], s0[i], x[i]);
+          store_sums(s, mine + a->width, x);
+        }
       }
     }
   }
-  float *mine = a.sums + (long)t * 4 * a.width;
-  if (a.want_sums[0]) store_sums(s, mine, sum_post);
-  if (a.want_sums[2]) store_sums(s, mine + 2 * a.width, sum_pre);
-  if constexpr (FULL) {
-    if (a.want_sums[1]) store_sums(s, mine + a.width, sum_post_bias);
-    if (a.want_sums[3]) store_sums(s, mine + 3 * a.width, sum_pre_bias);
+  float *mine = a0->sums + (unsigned long)t * 4 * a0->width;
+  if (a0->want_sums[2]) store_sums(s, mine + 2 * a0->width, p1);
+  if constexpr (BIAS) {
+    if (a0->want_sums[3]) store_sums(s, mine + 3 * a0->width, p0);
   }
 }
 
@@ -435,17 +540,17 @@ inline bool with_norm_shape(NormShape n, F &&f) {
     return true;                                                                           \
   }
   PCCL_NORM_SHAPE(64, 8)
-  PCCL_NORM_SHAPE(64, 16)
+  PCCL_NORM_SHAPE(128, 8)
   PCCL_NORM_SHAPE(256, 8)
-  PCCL_NORM_SHAPE(256, 16)
-  PCCL_NORM_SHAPE(512, 16)
+  PCCL_NORM_SHAPE(512, 8)
+  PCCL_NORM_SHAPE(1024, 8)
   PCCL_NORM_SHAPE(1024, 16)
 #undef PCCL_NORM_SHAPE
   return false;
 }
 
 template <int DT, bool PF32> hipError_t launch_fold_norm(NormShape n, hipStream_t stream, const ForwardArgs &a);
-template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool full, hipStream_t stream, const BackwardArgs &a);
+template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool bias, hipStream_t stream, const BackwardArgs &a);
 template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, hipStream_t stream, const SumsArgs &a);
 
 #define PCCL_DEFINE_FOLD_NORM(DT, PF32)                                                                                     \
@@ -458,12 +563,17 @@ template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, h
     });                                                                                                                     \
     return hipGetLastError();                                                                                               \
   }                                                                                                                         \
-  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool full, hipStream_t stream, const BackwardArgs &a) { \
+  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool bias, hipStream_t stream, const BackwardArgs &a) { \
     with_norm_shape(n, [&](auto l, auto e) {                                                                                \
       constexpr int L = decltype(l)::value, E = decltype(e)::value, kTeams = team_block(L) / L;                             \
       const unsigned grid = (a.n_teams + kTeams - 1) / kTeams;                                                              \
-      if (full) hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, L, E, true>), dim3(grid), dim3(team_block(L)), 0, stream, a); \
-      else hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, L, E, false>), dim3(grid), dim3(team_block(L)), 0, stream, a); \
+      const bool single = a.n_in == 1 && a.n_out <= 1;                                                                      \
+      auto run = [&](auto sg, auto b) {                                                                                     \
+        hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, L, E, decltype(sg)::value, decltype(b)::value>), dim3(grid), \
+                           dim3(team_block(L)), 0, stream, a);                                                              \
+      };                                                                                                                    \
+      if (single) bias ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});                \
+      else bias ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});                     \
     });                                                                                                                     \
     return hipGetLastError();                                                                                               \
   }                                                                                                                         \
