@@ -1,9 +1,11 @@
 // block_cache.hip -- pccl_hip_cache_write, pccl_hip_cache_read: keys and values coded in blocks of 32 elements with
 // a shared power-of-two scale as they are written to their pages, and read back through page tables.
 //
-// Four neighbouring lanes work on one block, eight elements each: 16 bytes of a 16-bit source a load, and the block's
-// largest magnitude is two data-parallel-primitive steps inside the quad away.  Blocks are numbered row by row
-// (row = token and head), so that consecutive quads walk a token's heads in memory order on both sides.
+// Four neighbouring lanes work on one block, eight elements each: 16 bytes of a 16-bit row a load or store, and the block's
+// largest magnitude is two data-parallel-primitive steps inside the quad away.  A lane keeps its head and its place in
+// the head for all tokens that its wavefront goes through, so that the multiplications which find them (quarter rate) are
+// paid once; where a token has 16 blocks or more, a wavefront works on one token at a time and finds slot, page and
+// addresses on the scalar unit.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -19,7 +21,8 @@ typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef unsigned int u32_a1 __attribute__((aligned(1)));
 
 constexpr int kQuad = 4, kPerLane = 8;  // lanes of a block, elements of a lane
-constexpr int kBlocksAtOnce = kBlock / kQuad;
+constexpr int kWaveBlocks = kWave / kQuad;
+constexpr int kWaves = kBlock / kWave;
 
 // n / d for n < 2^31 by a multiplication (Granlund and Montgomery's round-up method).
 struct Divisor {
@@ -35,132 +38,188 @@ struct Divisor {
 
 // ---- the formats ---------------------------------------------------------------------------------------
 // kTop: mantissa bits of the largest value as a binary32, kExponent: its exponent; kBits: of an element.
-// down(): eight scaled elements (none beyond the largest value) to 8 * kBits bits, nearest, ties to even.
 template <int FMT> struct CacheFormat;
-
-template <bool E5M2> struct CacheF8 {
-  static constexpr int kBits = 8;
-  static constexpr unsigned kTop = 0x600000u;  // 1.75 * 2^15 and 1.75 * 2^8
-  static constexpr int kExponent = E5M2 ? 15 : 8;
-  typedef F8Fmt<E5M2> F;
-  static __device__ __forceinline__ u32x2 down(const float *x) { return u32x2{F::down4(x[0], x[1], x[2], x[3]), F::down4(x[4], x[5], x[6], x[7])}; }
-  static __device__ __forceinline__ void up(u32x2 c, float scale, float *x) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const typename F::f32x2 lo = F::template up2<false>(c[w]), hi = F::template up2<true>(c[w]);
-      x[4 * w] = lo.x * scale;
-      x[4 * w + 1] = lo.y * scale;
-      x[4 * w + 2] = hi.x * scale;
-      x[4 * w + 3] = hi.y * scale;
-    }
-  }
+template <> struct CacheFormat<PCCL_CACHE_F8E4M3> {
+  static constexpr int kBits = 8, kExponent = 8;
+  static constexpr unsigned kTop = 0x600000u;  // 1.75 * 2^8
 };
-template <> struct CacheFormat<PCCL_CACHE_F8E4M3> : CacheF8<false> {};
-template <> struct CacheFormat<PCCL_CACHE_F8E5M2> : CacheF8<true> {};
-
+template <> struct CacheFormat<PCCL_CACHE_F8E5M2> {
+  static constexpr int kBits = 8, kExponent = 15;
+  static constexpr unsigned kTop = 0x600000u;  // 1.75 * 2^15
+};
 template <> struct CacheFormat<PCCL_CACHE_I8> {
-  static constexpr int kBits = 8;
+  static constexpr int kBits = 8, kExponent = 0;
   static constexpr unsigned kTop = 0x7e0000u;  // 127/64
-  static constexpr int kExponent = 0;
-  static __device__ __forceinline__ u32x2 down(const float *x) {
-    // 64 x + 1.5 * 2^23 is rounded to a whole number, whose low byte is the code (one fused step: one rounding);
-    // only a block whose scale would be 2^128 comes beyond 127
-    unsigned q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = as_u32(__builtin_fmaf(__builtin_amdgcn_fmed3f(x[i], -127.0f / 64, 127.0f / 64), 64.0f, 12582912.0f));
-    u32x2 c;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const unsigned lo = __builtin_amdgcn_perm(q[4 * w + 1], q[4 * w], 0x0c0c0400u), hi = __builtin_amdgcn_perm(q[4 * w + 3], q[4 * w + 2], 0x0c0c0400u);
-      c[w] = lo | hi << 16;
-    }
-    return c;
-  }
-  static __device__ __forceinline__ void up(u32x2 c, float scale, float *x) {
-    const float step = scale * (1.0f / 64);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)((int)(c[i / 4] << (24 - 8 * (i % 4))) >> 24) * step;
-  }
 };
-
 template <> struct CacheFormat<PCCL_CACHE_F4E2M1> {
-  static constexpr int kBits = 4;
+  static constexpr int kBits = 4, kExponent = 2;
   static constexpr unsigned kTop = 0x400000u;  // 1.5 * 2^2
-  static constexpr int kExponent = 2;
-  static __device__ __forceinline__ unsigned down(const float *x) {
-    unsigned c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], 1.0f, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], 1.0f, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], 1.0f, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], 1.0f, 3);
-    return c;
-  }
-  static __device__ __forceinline__ void up(unsigned c, float scale, float *x) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
-    x[0] = a.x * scale;
-    x[1] = a.y * scale;
-    x[2] = b.x * scale;
-    x[3] = b.y * scale;
-    x[4] = d.x * scale;
-    x[5] = d.y * scale;
-    x[6] = e.x * scale;
-    x[7] = e.y * scale;
-  }
 };
 
 // A lane's eight codes: two words or one.
 template <int BITS> struct LaneCodes { typedef u32x2 type; typedef u32x2_a1 any; };
 template <> struct LaneCodes<4> { typedef unsigned type; typedef u32_a1 any; };
 
-struct CacheArgs {
-  char *codes[PCCL_CACHE_MAX_TENSORS], *scales[PCCL_CACHE_MAX_TENSORS];
-  long code_page, code_token, code_head, scale_page, scale_token, scale_head;
-  long n_slots;
-  int heads, head_dim;
-  Divisor blocks, by_heads, page_tokens;  // blocks of a head, heads, tokens of a page
-};
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-struct WriteArgs : CacheArgs {
-  const char *srcs[PCCL_CACHE_MAX_TENSORS];
-  long src_token, src_head;  // bytes
-  const long *slots;
-  unsigned n_blocks;  // of the launch
-};
+// The 8- and 4-bit floats go through the scaled conversions (v_cvt_scalef32_pk_*): two elements an instruction, the scale's
+// exponent byte applied on the way, round to nearest even; checked over every code, scale byte and 16-bit source pattern.  The
+// format is a template argument of each, the word half or byte (an immediate) as well.
+#define PCCL_PACKED(T, x) __builtin_bit_cast(T, x)
+template <int DT, int FMT, int AT>
+__device__ __forceinline__ unsigned two_up(unsigned c, float scale) {  // codes AT * 2, AT * 2 + 1 of a word -> two 16-bit elements
+  if constexpr (DT == PCCL_BF16) {
+    if constexpr (FMT == PCCL_CACHE_F8E4M3) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, AT));
+    else if constexpr (FMT == PCCL_CACHE_F8E5M2) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(c, scale, AT));
+    else return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, AT));
+  } else {
+    if constexpr (FMT == PCCL_CACHE_F8E4M3) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, scale, AT));
+    else if constexpr (FMT == PCCL_CACHE_F8E5M2) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(c, scale, AT));
+    else return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, AT));
+  }
+}
+template <int FMT, int AT>
+__device__ __forceinline__ f32x2 two_up_f32(unsigned c, float scale) {
+  if constexpr (FMT == PCCL_CACHE_F8E4M3) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, scale, AT);
+  else if constexpr (FMT == PCCL_CACHE_F8E5M2) return __builtin_amdgcn_cvt_scalef32_pk_f32_bf8(c, scale, AT);
+  else return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, AT);
+}
+// two 16-bit elements into codes AT * 2, AT * 2 + 1 of word c
+template <int DT, int FMT, int AT>
+__device__ __forceinline__ unsigned two_down(unsigned c, unsigned w, float scale) {
+  if constexpr (DT == PCCL_BF16) {
+    const bf16x2 x = PCCL_PACKED(bf16x2, w);
+    if constexpr (FMT == PCCL_CACHE_F8E4M3) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(PCCL_PACKED(s16x2, c), x, scale, AT));
+    else if constexpr (FMT == PCCL_CACHE_F8E5M2) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(PCCL_PACKED(s16x2, c), x, scale, AT));
+    else return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, x, scale, AT);
+  } else {
+    const f16x2 x = PCCL_PACKED(f16x2, w);
+    if constexpr (FMT == PCCL_CACHE_F8E4M3) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(PCCL_PACKED(s16x2, c), x, scale, AT));
+    else if constexpr (FMT == PCCL_CACHE_F8E5M2) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(PCCL_PACKED(s16x2, c), x, scale, AT));
+    else return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, x, scale, AT);
+  }
+}
+template <int FMT, int AT>
+__device__ __forceinline__ unsigned two_down_f32(unsigned c, float a, float b, float scale) {
+  if constexpr (FMT == PCCL_CACHE_F8E4M3) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(PCCL_PACKED(s16x2, c), a, b, scale, AT));
+  else if constexpr (FMT == PCCL_CACHE_F8E5M2) return PCCL_PACKED(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(PCCL_PACKED(s16x2, c), a, b, scale, AT));
+  else return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, AT);
+}
+#undef PCCL_PACKED
 
-// The eight elements of a lane, from `at` on, `n` of them (0..8) inside the head; zeros behind.
-template <class R>
-struct Eight {
-  static constexpr int kPacks = 8 / R::kPack;
-  u32x4 v[kPacks];
-  __device__ __forceinline__ void load(const char *at, int n) {
-    if (n == 8) {
+// A lane's eight elements as they stand in memory.
+template <class R> struct Eight { u32x4 v[8 / R::kPack]; };
+
+// codes of scale byte s -> elements
+template <int DT, int FMT>
+__device__ __forceinline__ Eight<RowType<DT>> decode(typename LaneCodes<CacheFormat<FMT>::kBits>::type c, unsigned s) {
+  typedef RowType<DT> R;
+  Eight<R> e;
+  if constexpr (FMT == PCCL_CACHE_I8) {
+    // a scale's 64th is exact down to 2^-133, and so is its product with a whole number
+    const float step = as_f32(s == 255 ? 0x7fc00000u : s == 0 ? 0x400000u : s << 23) * (1.0f / 64);
+    float x[8];
 #pragma unroll
-      for (int j = 0; j < kPacks; ++j) v[j] = ((const typename R::pack_t *)at)[j];
+    for (int i = 0; i < 8; ++i) x[i] = (float)(signed char)(c[i / 4] >> (8 * (i % 4))) * step;
+#pragma unroll
+    for (int j = 0; j < 8 / R::kPack; ++j) e.v[j] = R::down(x + j * R::kPack);
+  } else {
+    const float scale = as_f32(s << 23);
+    unsigned w0, w1;  // words of codes 0-3 and 4-7; the 4-bit codes are all in one
+    if constexpr (CacheFormat<FMT>::kBits == 8) w0 = c[0], w1 = c[1];
+    else w0 = w1 = c;
+    constexpr int kNext = CacheFormat<FMT>::kBits == 8 ? 0 : 2;
+    if constexpr (DT == PCCL_F32) {
+      const f32x2 a = two_up_f32<FMT, 0>(w0, scale), b = two_up_f32<FMT, 1>(w0, scale);
+      const f32x2 d = two_up_f32<FMT, kNext>(w1, scale), f = two_up_f32<FMT, kNext + 1>(w1, scale);
+      e.v[0] = u32x4{as_u32(a.x), as_u32(a.y), as_u32(b.x), as_u32(b.y)};
+      e.v[1] = u32x4{as_u32(d.x), as_u32(d.y), as_u32(f.x), as_u32(f.y)};
     } else {
-#pragma unroll
-      for (int j = 0; j < kPacks; ++j) {
-        typename R::elem_t e[R::kPack];
-#pragma unroll
-        for (int i = 0; i < R::kPack; ++i) e[i] = j * R::kPack + i < n ? ((const typename R::elem_t *)at)[j * R::kPack + i] : (typename R::elem_t)0;
-        v[j] = __builtin_bit_cast(u32x4, e);
-      }
+      e.v[0] = u32x4{two_up<DT, FMT, 0>(w0, scale), two_up<DT, FMT, 1>(w0, scale), two_up<DT, FMT, kNext>(w1, scale), two_up<DT, FMT, kNext + 1>(w1, scale)};
     }
   }
-  __device__ __forceinline__ void up(float *x) const {
-#pragma unroll
-    for (int j = 0; j < kPacks; ++j) R::up(v[j], x + j * R::kPack);
-  }
-  // binary32 bits of the largest magnitude; magnitudes compare as whole numbers, infinities and NaN come out on top
-  __device__ __forceinline__ unsigned most() const {
+  return e;
+}
+
+// elements of a block with scale byte s -> codes; none passes the format's largest value, and a block of scale 255 has codes 0
+template <int DT, int FMT>
+__device__ __forceinline__ typename LaneCodes<CacheFormat<FMT>::kBits>::type encode(const Eight<RowType<DT>> &e, unsigned s) {
+  typedef RowType<DT> R;
+  typename LaneCodes<CacheFormat<FMT>::kBits>::type c{};
+  if constexpr (FMT == PCCL_CACHE_I8) {
     float x[8];
-    up(x);
+    unsigned q[8];
+#pragma unroll
+    for (int j = 0; j < 8 / R::kPack; ++j) R::up(e.v[j], x + j * R::kPack);
+    // 64 x / scale + 1.5 * 2^23 is rounded once, to a whole number, whose low byte is the code
+    if (s >= 6 && s < 254) {  // 64 / scale is a binary32, one fused step
+      const float f = as_f32((260u - s) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = as_u32(__builtin_fmaf(x[i], f, 12582912.0f));
+    } else {  // 1 / scale and 64 apart (exact; a subnormal product rounds to 0 either way); only here a block whose scale would be 2^128 saturates
+      const float f = as_f32(s == 254 ? 0x400000u : (254u - s) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = as_u32(__builtin_fmaf(__builtin_amdgcn_fmed3f(x[i] * f, -127.0f / 64, 127.0f / 64), 64.0f, 12582912.0f));
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const unsigned lo = __builtin_amdgcn_perm(q[4 * w + 1], q[4 * w], 0x0c0c0400u), hi = __builtin_amdgcn_perm(q[4 * w + 3], q[4 * w + 2], 0x04000c0cu);
+      c[w] = s == 255 ? 0 : lo | hi;
+    }
+  } else {
+    const float scale = as_f32(s << 23);
+    unsigned w0 = 0, w1 = 0;
+    if constexpr (DT == PCCL_F32) {
+      const u32x4 a = e.v[0], b = e.v[1];
+      w0 = two_down_f32<FMT, 0>(w0, as_f32(a[0]), as_f32(a[1]), scale);
+      w0 = two_down_f32<FMT, 1>(w0, as_f32(a[2]), as_f32(a[3]), scale);
+      if constexpr (CacheFormat<FMT>::kBits == 8) {
+        w1 = two_down_f32<FMT, 0>(w1, as_f32(b[0]), as_f32(b[1]), scale);
+        w1 = two_down_f32<FMT, 1>(w1, as_f32(b[2]), as_f32(b[3]), scale);
+      } else {
+        w0 = two_down_f32<FMT, 2>(w0, as_f32(b[0]), as_f32(b[1]), scale);
+        w0 = two_down_f32<FMT, 3>(w0, as_f32(b[2]), as_f32(b[3]), scale);
+      }
+    } else {
+      const u32x4 a = e.v[0];
+      const unsigned a0 = a[0], a1 = a[1], a2 = a[2], a3 = a[3];
+      w0 = two_down<DT, FMT, 0>(w0, a0, scale);
+      w0 = two_down<DT, FMT, 1>(w0, a1, scale);
+      if constexpr (CacheFormat<FMT>::kBits == 8) {
+        w1 = two_down<DT, FMT, 0>(w1, a2, scale);
+        w1 = two_down<DT, FMT, 1>(w1, a3, scale);
+      } else {
+        w0 = two_down<DT, FMT, 2>(w0, a2, scale);
+        w0 = two_down<DT, FMT, 3>(w0, a3, scale);
+      }
+    }
+    if (s == 255) w0 = w1 = 0;
+    if constexpr (CacheFormat<FMT>::kBits == 8) c = u32x2{w0, w1};
+    else c = w0;
+  }
+  return c;
+}
+
+// binary32 bits of the largest magnitude of a lane's elements; magnitudes compare as whole numbers, infinities and NaN come out on top
+template <int DT>
+__device__ __forceinline__ unsigned most_of(const Eight<RowType<DT>> &e) {
+  if constexpr (DT == PCCL_F32) {
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, as_u32(x[i]) & 0x7fffffffu);
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max(m, e.v[j][i] & 0x7fffffffu);
     return m;
+  } else {
+    const u32x4 v = e.v[0] & 0x7fff7fffu;
+    const unsigned v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+    const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v0), __builtin_bit_cast(u16x2, v1));
+    const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v2), __builtin_bit_cast(u16x2, v3));
+    const u16x2 m = __builtin_elementwise_max(a, b);
+    return as_u32(RowType<DT>::up1(max(m.x, m.y)));
   }
-};
+}
 
 __device__ __forceinline__ unsigned quad_max(unsigned m) {
   m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
@@ -178,53 +237,118 @@ __device__ __forceinline__ unsigned scale_of(unsigned most) {
   return most >= 0x7f800000u ? 255u : (unsigned)s;
 }
 
-template <int DT, int FMT, int TIMES>
+struct CacheArgs {
+  char *codes[PCCL_CACHE_MAX_TENSORS], *scales[PCCL_CACHE_MAX_TENSORS];
+  long code_page, code_token, code_head, scale_page, scale_token, scale_head;
+  long row_head;            // bytes from one head of a source or output row to the next
+  int head_dim;
+  unsigned blocks;          // of a token: heads times blocks of a head
+  unsigned group;           // tokens that a wavefront has side by side (1 from 16 blocks on)
+  Divisor by_blocks, head_blocks, page_tokens, chunks;  // blocks of a token; of a head; tokens of a page; wavefronts' shares of a token
+};
+
+// Where a lane stands: its token among those side by side, its head's and block's offsets.
+struct Place {
+  bool on;
+  unsigned token, block;
+  int n, q;               // elements inside the head (0..8), lane of the quad
+  long code, scale, row;  // bytes behind the token's start
+};
+template <bool ONE>  // one token at a time
+__device__ __forceinline__ Place place_of(const CacheArgs &a, unsigned chunk, int bits, int elem_bytes) {
+  Place p;
+  const unsigned lane = threadIdx.x % kWave, at = lane / kQuad;
+  p.q = (int)(lane % kQuad);
+  p.token = ONE ? 0 : a.by_blocks.divide(at);
+  const unsigned r = ONE ? chunk * kWaveBlocks + at : at - p.token * a.blocks;
+  p.on = ONE ? r < a.blocks : p.token < a.group;
+  const unsigned head = a.head_blocks.divide(r);
+  p.block = r - head * a.head_blocks.d;
+  const int first = (int)p.block * PCCL_CACHE_BLOCK + p.q * kPerLane;
+  p.n = min(max(a.head_dim - first, 0), kPerLane);
+  p.code = (long)head * a.code_head + first * bits / 8;
+  p.scale = (long)head * a.scale_head + p.block;
+  p.row = (long)head * a.row_head + first * elem_bytes;
+  return p;
+}
+
+// eight elements from `at` on, n of them there, zeros behind
+template <class R>
+__device__ __forceinline__ Eight<R> load_eight(const char *at, int n) {
+  Eight<R> e;
+#pragma unroll
+  for (int j = 0; j < 8 / R::kPack; ++j) {
+    if (n == 8) {
+      e.v[j] = ((const typename R::pack_t *)at)[j];
+    } else {
+      typename R::elem_t x[R::kPack];
+#pragma unroll
+      for (int i = 0; i < R::kPack; ++i) x[i] = j * R::kPack + i < n ? ((const typename R::elem_t *)at)[j * R::kPack + i] : (typename R::elem_t)0;
+      e.v[j] = __builtin_bit_cast(u32x4, x);
+    }
+  }
+  return e;
+}
+template <class R>
+__device__ __forceinline__ void store_eight(char *at, int n, const Eight<R> &e) {
+#pragma unroll
+  for (int j = 0; j < 8 / R::kPack; ++j) {
+    if (n == 8) {
+      ((typename R::pack_t *)at)[j] = e.v[j];
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::kPack; ++i)
+        if (j * R::kPack + i < n) {
+          const unsigned w = e.v[j][i * R::kBytes / 4];
+          ((typename R::elem_t *)at)[j * R::kPack + i] = (typename R::elem_t)(R::kBytes == 2 && i % 2 ? w >> 16 : w);
+        }
+    }
+  }
+}
+
+struct WriteArgs : CacheArgs {
+  const char *srcs[PCCL_CACHE_MAX_TENSORS];
+  long src_token;  // bytes
+  const long *slots;
+  unsigned long n_slots;
+  unsigned tokens;  // of the launch
+};
+
+template <int DT, int FMT, int TIMES, bool ONE>
 __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) {
   typedef RowType<DT> R;
   typedef CacheFormat<FMT> F;
   typedef LaneCodes<F::kBits> L;
+  const unsigned wave = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const unsigned tile = a.chunks.divide(wave), chunk = wave - tile * a.chunks.d;
+  const unsigned token0 = tile * TIMES * a.group;
+  if (token0 >= a.tokens) return;
+  const Place p = place_of<ONE>(a, chunk, F::kBits, R::kBytes);
   const char *src = a.srcs[blockIdx.y];
   char *codes = a.codes[blockIdx.y], *scales = a.scales[blockIdx.y];
-  const int q = (int)threadIdx.x % kQuad;
+  unsigned long slot[TIMES];
   Eight<R> e[TIMES];
-  long slot[TIMES];
-  unsigned block[TIMES], head[TIMES];
-  int n[TIMES];
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    const unsigned u = (blockIdx.x * TIMES + t) * kBlocksAtOnce + threadIdx.x / kQuad;
-    slot[t] = -1;
-    if (u < a.n_blocks) {
-      const unsigned row = a.blocks.divide(u), token = a.by_heads.divide(row);
-      block[t] = u - row * a.blocks.d;
-      head[t] = row - token * a.by_heads.d;
-      slot[t] = a.slots[token];
-      const int first = (int)block[t] * PCCL_CACHE_BLOCK + q * kPerLane;
-      n[t] = min(max(a.head_dim - first, 0), kPerLane);
-      if ((unsigned long)slot[t] < (unsigned long)a.n_slots)
-        e[t].load(src + token * a.src_token + head[t] * a.src_head + (long)first * R::kBytes, n[t]);
-      else slot[t] = -1;
-    }
+    const unsigned token = token0 + t * a.group + p.token;
+    const bool there = token < a.tokens;
+    slot[t] = (unsigned long)a.slots[there ? token : 0];  // (no branch around the load: all of them go out together)
+    if (!there) slot[t] = ~0ul;
   }
 #pragma unroll
-  for (int t = 0; t < TIMES; ++t) {
-    if (slot[t] < 0) continue;  // whole quads
-    const unsigned s = scale_of<F>(quad_max(e[t].most()));
-    float x[8];
-    e[t].up(x);
-    // 2^(127 - s); exact, and so is the product (a subnormal product is far below half of the smallest code)
-    const float inverse = as_f32(s == 255 ? 0u : s == 254 ? 0x400000u : (254u - s) << 23);
+  for (int t = 0; t < TIMES; ++t)
+    if (slot[t] < a.n_slots && p.on) e[t] = load_eight<R>(src + (unsigned long)(token0 + t * a.group + p.token) * a.src_token + p.row, p.n);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= inverse;
-    typename L::type c = F::down(x);
-    if (s == 255) c = typename L::type{};
+  for (int t = 0; t < TIMES; ++t) {
+    if (slot[t] >= a.n_slots || !p.on) continue;  // whole quads
+    const unsigned s = scale_of<F>(quad_max(most_of<DT>(e[t])));
+    const typename L::type c = encode<DT, FMT>(e[t], s);
     const unsigned page = a.page_tokens.divide((unsigned)slot[t]), token = (unsigned)slot[t] - page * a.page_tokens.d;
-    char *to = codes + page * a.code_page + token * a.code_token + head[t] * a.code_head +
-               (block[t] * PCCL_CACHE_BLOCK + q * kPerLane) * F::kBits / 8;
-    if (n[t] == 8) {
+    char *to = codes + ((unsigned long)page * a.code_page + (unsigned long)token * a.code_token) + p.code;
+    if (p.n == 8) {
       *(typename L::any *)to = c;
     } else {
-      const int bytes = (n[t] * F::kBits + 7) / 8;
+      const int bytes = (p.n * F::kBits + 7) / 8;
 #pragma unroll
       for (int i = 0; i < F::kBits; ++i) {
         unsigned w;
@@ -233,61 +357,57 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
         if (i < bytes) to[i] = (char)(w >> (8 * (i % 4)));
       }
     }
-    if (q == 0) scales[page * a.scale_page + token * a.scale_token + head[t] * a.scale_head + block[t]] = (char)s;
+    if (p.q == 0) scales[((unsigned long)page * a.scale_page + (unsigned long)token * a.scale_token) + p.scale] = (char)s;
   }
 }
 
 struct ReadArgs : CacheArgs {
   char *outs[PCCL_CACHE_MAX_TENSORS];
-  long out_token, out_head;  // bytes
-  long out_rows, max_len, table_stride;
+  long out_token;  // bytes
+  long out_rows, max_len, table_stride, n_pages;
   const int *page_table, *lengths;
   const long *row_start;
-  long token0;        // the launch's first token of every sequence
-  unsigned n_blocks;  // of the launch, per sequence
+  unsigned token0;  // the launch's first token of every sequence
   int seq0;
-  long n_pages;
 };
 
-template <int DT, int FMT, int TIMES>
+template <int DT, int FMT, int TIMES, bool ONE>
 __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
   typedef RowType<DT> R;
   typedef CacheFormat<FMT> F;
   typedef LaneCodes<F::kBits> L;
   const long seq = a.seq0 + (long)blockIdx.y;
-  const char *codes = a.codes[blockIdx.z], *scales = a.scales[blockIdx.z];
-  char *out = a.outs[blockIdx.z];
-  const int q = (int)threadIdx.x % kQuad;
+  const unsigned wave = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const unsigned tile = a.chunks.divide(wave), chunk = wave - tile * a.chunks.d;
+  const unsigned long token0 = a.token0 + (unsigned long)tile * TIMES * a.group;
   long length = a.lengths[seq];
   if (length > a.max_len) length = a.max_len;
-  const unsigned base = blockIdx.x * TIMES * kBlocksAtOnce;
-  if (a.token0 + (long)a.by_heads.divide(a.blocks.divide(base)) >= length) return;  // the workgroup's first token is behind the end
+  if ((long)token0 >= length) return;
+  const Place p = place_of<ONE>(a, chunk, F::kBits, R::kBytes);
+  const char *codes = a.codes[blockIdx.z], *scales = a.scales[blockIdx.z];
+  char *out = a.outs[blockIdx.z];
   const long first_row = a.row_start ? a.row_start[seq] : seq * a.max_len;
   const int *table = a.page_table + seq * a.table_stride;
+  unsigned long page[TIMES];
   typename L::type c[TIMES];
   unsigned s[TIMES];
-  char *to[TIMES];
-  int n[TIMES];
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    const unsigned u = base + t * kBlocksAtOnce + threadIdx.x / kQuad;
-    n[t] = 0;
-    if (u >= a.n_blocks) continue;
-    const unsigned row = a.blocks.divide(u), token_of = a.by_heads.divide(row);
-    const unsigned block = u - row * a.blocks.d, head = row - token_of * a.by_heads.d;
-    const long pos = a.token0 + token_of, out_row = first_row + pos;
-    const unsigned entry = a.page_tokens.divide((unsigned)pos);
-    if (pos >= length || (long)entry >= a.table_stride || (unsigned long)out_row >= (unsigned long)a.out_rows) continue;
-    const long page = table[entry];
-    if ((unsigned long)page >= (unsigned long)a.n_pages) continue;
-    const unsigned token = (unsigned)pos - entry * a.page_tokens.d;
-    const int first = (int)block * PCCL_CACHE_BLOCK + q * kPerLane;
-    n[t] = min(max(a.head_dim - first, 0), kPerLane);
-    const char *from = codes + page * a.code_page + token * a.code_token + head * a.code_head + (long)first * F::kBits / 8;
-    if (n[t] == 8) {
+    const unsigned pos = (unsigned)token0 + t * a.group + p.token, entry = a.page_tokens.divide(pos);
+    const bool named = (long)pos < length && (long)entry < a.table_stride && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows;
+    page[t] = (unsigned long)(long)table[named ? entry : 0];  // (no branch around the load: all of them go out together)
+    if (!named) page[t] = ~0ul;
+  }
+#pragma unroll
+  for (int t = 0; t < TIMES; ++t) {
+    if (page[t] >= (unsigned long)a.n_pages || !p.on) continue;
+    const unsigned pos = (unsigned)token0 + t * a.group + p.token, token = pos - a.page_tokens.divide(pos) * a.page_tokens.d;
+    const char *from = codes + (page[t] * a.code_page + (unsigned long)token * a.code_token) + p.code;
+    s[t] = (unsigned char)(scales + (page[t] * a.scale_page + (unsigned long)token * a.scale_token))[p.scale];
+    if (p.n == 8) {
       c[t] = *(const typename L::any *)from;
     } else {
-      const int bytes = (n[t] * F::kBits + 7) / 8;
+      const int bytes = (p.n * F::kBits + 7) / 8;
       unsigned w[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < F::kBits; ++i)
@@ -295,23 +415,12 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
       if constexpr (F::kBits == 8) c[t] = u32x2{w[0], w[1]};
       else c[t] = w[0];
     }
-    s[t] = (unsigned char)scales[page * a.scale_page + token * a.scale_token + head * a.scale_head + block];
-    to[t] = out + out_row * a.out_token + head * a.out_head + (long)first * R::kBytes;
   }
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    if (n[t] == 0) continue;
-    float x[8];
-    // (every product is exact in binary32: a code has at most 7 bits, the smallest is 2^-16 of its scale)
-    F::up(c[t], as_f32(s[t] == 255 ? 0x7fc00000u : s[t] == 0 ? 0x400000u : s[t] << 23), x);
-    if (n[t] == 8) {
-#pragma unroll
-      for (int j = 0; j < 8 / R::kPack; ++j) ((typename R::pack_t *)to[t])[j] = R::down(x + j * R::kPack);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n[t]) ((typename R::elem_t *)to[t])[i] = R::down1(x[i]);
-    }
+    if (page[t] >= (unsigned long)a.n_pages || !p.on) continue;
+    const unsigned pos = (unsigned)token0 + t * a.group + p.token;
+    store_eight<R>(out + (unsigned long)(first_row + pos) * a.out_token + p.row, p.n, decode<DT, FMT>(c[t], s[t]));
   }
 }
 
@@ -369,12 +478,13 @@ int check_cache(const pccl_cache_desc *c, int dtype, const void *const *tensors,
   a->scale_page = c->scale_page;
   a->scale_token = c->scale_token;
   a->scale_head = c->scale_head;
-  a->n_slots = c->n_pages * c->page_tokens;
-  a->heads = c->heads;
   a->head_dim = c->head_dim;
-  a->blocks.set((unsigned)blocks);
-  a->by_heads.set((unsigned)c->heads);
+  a->blocks = (unsigned)c->heads * (unsigned)blocks;  // at most 2^27
+  a->group = std::max(1u, kWaveBlocks / a->blocks);
+  a->by_blocks.set(a->blocks);
+  a->head_blocks.set((unsigned)blocks);
   a->page_tokens.set((unsigned)c->page_tokens);
+  a->chunks.set(a->group > 1 ? 1 : (a->blocks + kWaveBlocks - 1) / kWaveBlocks);
   return PCCL_OK;
 }
 
@@ -393,10 +503,28 @@ void with_types(int dtype, int format, F &&f) {
   else of_format(std::integral_constant<int, PCCL_F16>{});
 }
 
-constexpr int kTimes = 4;  // blocks a quad has in flight where there are enough of them
+constexpr int kTimes = 4;  // groups of tokens that a wavefront has in flight where there are enough of them
 
-// whether n blocks give every compute unit eight workgroups of kTimes blocks a quad
-bool many(long n) { return n >= (long)pccl_host::compute_units() * 8 * kBlocksAtOnce * kTimes; }
+// whether n wavefronts' worth of tokens give every compute unit eight workgroups of kTimes groups a wavefront
+bool many(long n) { return n >= (long)pccl_host::compute_units() * 8 * kWaves * kTimes; }
+
+// Tokens of a launch: wavefronts stay below 2^26 (a grid times its lanes must fit 32 bits) and below what Divisor divides.
+long launch_tokens(const CacheArgs &a) { return std::max(1l, (1l << 26) / a.chunks.d); }
+
+// Workgroups of a launch over n tokens.
+unsigned workgroups(const CacheArgs &a, long tokens, int times) {
+  const long tiles = (tokens + (long)times * a.group - 1) / ((long)times * a.group);
+  return (unsigned)((tiles * a.chunks.d + kWaves - 1) / kWaves);
+}
+
+// Calls f(times, one token at a time) with both as constants.
+template <class F>
+void with_shape(bool four, bool one, F &&f) {
+  typedef std::integral_constant<int, kTimes> Four;
+  typedef std::integral_constant<int, 1> Once;
+  if (four) one ? f(Four{}, std::true_type{}) : f(Four{}, std::false_type{});
+  else one ? f(Once{}, std::true_type{}) : f(Once{}, std::false_type{});
+}
 
 int launched(const char *what) {
   const hipError_t e = hipGetLastError();
@@ -423,18 +551,20 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
   if (tokens == 0 || c->n_pages == 0) return PCCL_OK;
   const int es = pccl_host::pccl_dtype_bytes(dtype);
   a.src_token = src_token_stride * es;
-  a.src_head = src_head_stride * es;
-  const long per_token = (long)c->heads * a.blocks.d, most = 0x7fffffffl / per_token;  // block numbers of a launch stay below 2^31
+  a.row_head = src_head_stride * es;
+  a.n_slots = (unsigned long)(c->n_pages * c->page_tokens);
+  const long most = launch_tokens(a);
   for (long lo = 0; lo < tokens; lo += most) {
     const long n = std::min(most, tokens - lo);
     for (int k = 0; k < c->n_tensors; ++k) a.srcs[k] = (const char *)srcs[k] + lo * a.src_token;
     a.slots = slots + lo;
-    a.n_blocks = (unsigned)(n * per_token);
+    a.tokens = (unsigned)n;
+    const bool four = many((n + a.group - 1) / a.group * a.chunks.d * c->n_tensors);
     with_types(dtype, c->format, [&](auto t, auto f) {
-      constexpr int DT = decltype(t)::value, FMT = decltype(f)::value;
-      auto grid = [&](unsigned times) { return dim3((a.n_blocks + kBlocksAtOnce * times - 1) / (kBlocksAtOnce * times), c->n_tensors); };
-      if (many((long)a.n_blocks * c->n_tensors)) hipLaunchKernelGGL((cache_write_kernel<DT, FMT, kTimes>), grid(kTimes), dim3(kBlock), 0, (hipStream_t)stream, a);
-      else hipLaunchKernelGGL((cache_write_kernel<DT, FMT, 1>), grid(1), dim3(kBlock), 0, (hipStream_t)stream, a);
+      with_shape(four, a.group == 1, [&](auto times, auto one) {
+        hipLaunchKernelGGL((cache_write_kernel<decltype(t)::value, decltype(f)::value, decltype(times)::value, decltype(one)::value>),
+                           dim3(workgroups(a, n, decltype(times)::value), c->n_tensors), dim3(kBlock), 0, (hipStream_t)stream, a);
+      });
     });
     rc = launched("cache_write");
     if (rc != PCCL_OK) return rc;
@@ -467,7 +597,7 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
   const int es = pccl_host::pccl_dtype_bytes(dtype);
   for (int k = 0; k < c->n_tensors; ++k) a.outs[k] = (char *)outs[k];
   a.out_token = out_token_stride * es;
-  a.out_head = out_head_stride * es;
+  a.row_head = out_head_stride * es;
   a.out_rows = out_rows;
   a.max_len = max_len;
   a.page_table = page_table;
@@ -475,18 +605,19 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
   a.lengths = lengths;
   a.row_start = row_start;
   a.n_pages = c->n_pages;
-  const long per_token = (long)c->heads * a.blocks.d, most = 0x7fffffffl / per_token;
+  const long most = launch_tokens(a);
   for (int seq = 0; seq < n_seq; seq += 65535) {
     a.seq0 = seq;
     const int seqs = std::min(65535, n_seq - seq);
     for (long lo = 0; lo < max_len; lo += most) {
-      a.token0 = lo;
-      a.n_blocks = (unsigned)(std::min(most, max_len - lo) * per_token);
+      a.token0 = (unsigned)lo;
+      const long n = std::min(most, max_len - lo);
+      const bool four = many((n + a.group - 1) / a.group * a.chunks.d * seqs * c->n_tensors);
       with_types(dtype, c->format, [&](auto t, auto f) {
-        constexpr int DT = decltype(t)::value, FMT = decltype(f)::value;
-        auto grid = [&](unsigned times) { return dim3((a.n_blocks + kBlocksAtOnce * times - 1) / (kBlocksAtOnce * times), seqs, c->n_tensors); };
-        if (many((long)a.n_blocks * seqs * c->n_tensors)) hipLaunchKernelGGL((cache_read_kernel<DT, FMT, kTimes>), grid(kTimes), dim3(kBlock), 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((cache_read_kernel<DT, FMT, 1>), grid(1), dim3(kBlock), 0, (hipStream_t)stream, a);
+        with_shape(four, a.group == 1, [&](auto times, auto one) {
+          hipLaunchKernelGGL((cache_read_kernel<decltype(t)::value, decltype(f)::value, decltype(times)::value, decltype(one)::value>),
+                             dim3(workgroups(a, n, decltype(times)::value), seqs, c->n_tensors), dim3(kBlock), 0, (hipStream_t)stream, a);
+        });
       });
       rc = launched("cache_read");
       if (rc != PCCL_OK) return rc;

@@ -122,3 +122,47 @@ def test_read(hip, fmt, dtype, layout):
                     if page_of < pages:
                         want[start[s] + t, :, :dim] = ref.decode(fmt, codes[page_of, t % page], scales[page_of, t % page], dim, dtype)
             assert ref.same(outs[k], want), "%s %s %s heads %d dim %d tensor %d" % (fmt, dtype, layout, heads, dim, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_code_with_every_scale(hip, fmt, dtype):
+    """256 tokens with one scale byte each, every code in each of them."""
+    import torch
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1, 1).contiguous()
+    dim = 256 if ref.BITS[fmt] == 8 else 512
+    scales = torch.arange(256, dtype=torch.uint8)[:, None, None].expand(-1, -1, dim // 32).contiguous()
+    cache = hip.Cache(fmt, 1, dim, 256, 1, [codes.cuda()], [scales.cuda()])
+    out = torch.zeros(256, 1, dim, dtype=ref.TYPES[dtype], device="cuda")
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([256], dtype=torch.int32, device="cuda")
+    cache.read(dtype, [out], table, lengths, 1, 256)
+    torch.cuda.synchronize()
+    assert ref.same(out, ref.decode(fmt, codes, scales, dim, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_pattern_under_scales_near_its_own(hip, fmt, dtype):
+    """All 65536 patterns of a 16-bit type, 31 to a block in the order of their magnitude, each block with one element that is the
+    largest of them times 1, 1.5, 2, ... 2^8 and sets the scale."""
+    import torch
+    t = ref.TYPES[dtype]
+    bits = torch.arange(65536, dtype=torch.int32)
+    order = torch.argsort((bits & 0x7fff) * 2 + (bits >> 15))
+    patterns = torch.cat([bits[order], bits[order][-(-65536 % 31):]]).to(torch.int16).view(t).view(-1, 31)
+    most = torch.where(torch.isfinite(patterns), patterns.double().abs(), 0.0).amax(-1)
+    blocks = []
+    for k in range(9):
+        for f in (1.0, 1.5):
+            lead = (most * f * 2.0 ** k).clamp(max=float(torch.finfo(t).max)).to(t)
+            blocks.append(torch.cat([lead[:, None], patterns], 1))
+    x = torch.cat(blocks)[:, None, :].contiguous()  # tokens x 1 head x 32
+    n = x.shape[0]
+    codes, scales = ref.encode(fmt, x.double())
+    row = codes.shape[-1]
+    dev_codes, dev_scales = torch.zeros(n, 1, 1, row, dtype=torch.uint8, device="cuda"), torch.zeros(n, 1, 1, 1, dtype=torch.uint8, device="cuda")
+    hip.Cache(fmt, 1, 32, 1, n, [dev_codes], [dev_scales]).write(dtype, [x.cuda()], torch.arange(n, device="cuda"), n)
+    torch.cuda.synchronize()
+    assert torch.equal(dev_scales.cpu().view(n, 1, 1), scales)
+    off = (dev_codes.cpu().view(n, row) != codes.view(n, row)).any(-1)
+    assert not bool(off.any()), "%d of %d blocks, first %s" % (int(off.sum()), n, x[off][0])
