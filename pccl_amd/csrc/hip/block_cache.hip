@@ -1,11 +1,11 @@
 // block_cache.hip -- pccl_hip_cache_write, pccl_hip_cache_read: keys and values coded in blocks of 32 elements with
 // a shared power-of-two scale as they are written to their pages, and read back through page tables.
 //
-// Four neighbouring lanes work on one block, eight elements each: 16 bytes of a 16-bit row a load or store, and the block's
-// largest magnitude is two data-parallel-primitive steps inside the quad away.  A lane keeps its head and its place in
+// A lane works on 16 bytes of a row: four neighbouring lanes on one block of a 16-bit row, eight on one of binary32, so that the
+// block's largest magnitude is two or three data-parallel-primitive steps away.  A lane keeps its head and its place in
 // the head for all tokens that its wavefront goes through, so that the multiplications which find them (quarter rate) are
-// paid once; where a token has 16 blocks or more, a wavefront works on one token at a time and finds slot, page and
-// addresses on the scalar unit.
+// paid once; where a token fills a wavefront, it works on one token at a time and finds slot, page and
+// addresses on the scalar unit.  (Reading needs no block's lanes side by side: there a short last block takes only the lanes it fills.)
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
@@ -19,9 +19,8 @@ namespace pccl_dev {
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef unsigned int u32_a1 __attribute__((aligned(1)));
+typedef unsigned short u16_a1 __attribute__((aligned(1)));
 
-constexpr int kQuad = 4, kPerLane = 8;  // lanes of a block, elements of a lane
-constexpr int kWaveBlocks = kWave / kQuad;
 constexpr int kWaves = kBlock / kWave;
 
 // n / d for n < 2^31 by a multiplication (Granlund and Montgomery's round-up method).
@@ -56,9 +55,13 @@ template <> struct CacheFormat<PCCL_CACHE_F4E2M1> {
   static constexpr unsigned kTop = 0x400000u;  // 1.5 * 2^2
 };
 
-// A lane's eight codes: two words or one.
-template <int BITS> struct LaneCodes { typedef u32x2 type; typedef u32x2_a1 any; };
-template <> struct LaneCodes<4> { typedef unsigned type; typedef u32_a1 any; };
+// A lane's codes: eight of 8 bits in two words, or as many as there are in the low bits of one.
+template <int BITS> struct LaneCodes { typedef unsigned type; };
+template <> struct LaneCodes<64> { typedef u32x2 type; };
+template <int BITS> struct StoredCodes;
+template <> struct StoredCodes<64> { typedef u32x2_a1 type; };
+template <> struct StoredCodes<32> { typedef u32_a1 type; };
+template <> struct StoredCodes<16> { typedef u16_a1 type; };
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -108,111 +111,137 @@ __device__ __forceinline__ unsigned two_down_f32(unsigned c, float a, float b, f
 }
 #undef PCCL_PACKED
 
-// A lane's eight elements as they stand in memory.
-template <class R> struct Eight { u32x4 v[8 / R::kPack]; };
-
-// codes of scale byte s -> elements
 template <int DT, int FMT>
-__device__ __forceinline__ Eight<RowType<DT>> decode(typename LaneCodes<CacheFormat<FMT>::kBits>::type c, unsigned s) {
+struct Lane {
   typedef RowType<DT> R;
-  Eight<R> e;
-  if constexpr (FMT == PCCL_CACHE_I8) {
-    // a scale's 64th is exact down to 2^-133, and so is its product with a whole number
-    const float step = as_f32(s == 255 ? 0x7fc00000u : s == 0 ? 0x400000u : s << 23) * (1.0f / 64);
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)(signed char)(c[i / 4] >> (8 * (i % 4))) * step;
-#pragma unroll
-    for (int j = 0; j < 8 / R::kPack; ++j) e.v[j] = R::down(x + j * R::kPack);
-  } else {
-    const float scale = as_f32(s << 23);
-    unsigned w0, w1;  // words of codes 0-3 and 4-7; the 4-bit codes are all in one
-    if constexpr (CacheFormat<FMT>::kBits == 8) w0 = c[0], w1 = c[1];
+  static constexpr int kElems = R::kPack, kBits = kElems * CacheFormat<FMT>::kBits;
+  static constexpr int kBlockLanes = PCCL_CACHE_BLOCK / kElems;
+  typedef typename LaneCodes<kBits>::type Codes;
+
+  // codes of scale byte s -> elements as they stand in memory
+  static __device__ __forceinline__ u32x4 decode(Codes c, unsigned s) {
+    unsigned w0, w1;  // the words that elements 0-3 and 4-7 are in
+    if constexpr (kBits == 64) w0 = c[0], w1 = c[1];
     else w0 = w1 = c;
-    constexpr int kNext = CacheFormat<FMT>::kBits == 8 ? 0 : 2;
-    if constexpr (DT == PCCL_F32) {
-      const f32x2 a = two_up_f32<FMT, 0>(w0, scale), b = two_up_f32<FMT, 1>(w0, scale);
-      const f32x2 d = two_up_f32<FMT, kNext>(w1, scale), f = two_up_f32<FMT, kNext + 1>(w1, scale);
-      e.v[0] = u32x4{as_u32(a.x), as_u32(a.y), as_u32(b.x), as_u32(b.y)};
-      e.v[1] = u32x4{as_u32(d.x), as_u32(d.y), as_u32(f.x), as_u32(f.y)};
+    if constexpr (FMT == PCCL_CACHE_I8) {
+      // a scale's 64th is exact down to 2^-133, and so is its product with a whole number
+      const float step = as_f32(s == 255 ? 0x7fc00000u : s == 0 ? 0x400000u : s << 23) * (1.0f / 64);
+      float x[kElems];
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) x[i] = (float)(signed char)((i < 4 ? w0 : w1) >> (8 * (i % 4))) * step;
+      return R::down(x);
     } else {
-      e.v[0] = u32x4{two_up<DT, FMT, 0>(w0, scale), two_up<DT, FMT, 1>(w0, scale), two_up<DT, FMT, kNext>(w1, scale), two_up<DT, FMT, kNext + 1>(w1, scale)};
+      const float scale = as_f32(s << 23);
+      if constexpr (DT == PCCL_F32) {
+        const f32x2 a = two_up_f32<FMT, 0>(w0, scale), b = two_up_f32<FMT, 1>(w0, scale);
+        return u32x4{as_u32(a.x), as_u32(a.y), as_u32(b.x), as_u32(b.y)};
+      } else {
+        constexpr int kNext = kBits == 64 ? 0 : 2;
+        return u32x4{two_up<DT, FMT, 0>(w0, scale), two_up<DT, FMT, 1>(w0, scale), two_up<DT, FMT, kNext>(w1, scale), two_up<DT, FMT, kNext + 1>(w1, scale)};
+      }
     }
   }
-  return e;
-}
 
-// elements of a block with scale byte s -> codes; none passes the format's largest value, and a block of scale 255 has codes 0
-template <int DT, int FMT>
-__device__ __forceinline__ typename LaneCodes<CacheFormat<FMT>::kBits>::type encode(const Eight<RowType<DT>> &e, unsigned s) {
-  typedef RowType<DT> R;
-  typename LaneCodes<CacheFormat<FMT>::kBits>::type c{};
-  if constexpr (FMT == PCCL_CACHE_I8) {
-    float x[8];
-    unsigned q[8];
-#pragma unroll
-    for (int j = 0; j < 8 / R::kPack; ++j) R::up(e.v[j], x + j * R::kPack);
-    // 64 x / scale + 1.5 * 2^23 is rounded once, to a whole number, whose low byte is the code
-    if (s >= 6 && s < 254) {  // 64 / scale is a binary32, one fused step
-      const float f = as_f32((260u - s) << 23);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = as_u32(__builtin_fmaf(x[i], f, 12582912.0f));
-    } else {  // 1 / scale and 64 apart (exact; a subnormal product rounds to 0 either way); only here a block whose scale would be 2^128 saturates
-      const float f = as_f32(s == 254 ? 0x400000u : (254u - s) << 23);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = as_u32(__builtin_fmaf(__builtin_amdgcn_fmed3f(x[i] * f, -127.0f / 64, 127.0f / 64), 64.0f, 12582912.0f));
-    }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const unsigned lo = __builtin_amdgcn_perm(q[4 * w + 1], q[4 * w], 0x0c0c0400u), hi = __builtin_amdgcn_perm(q[4 * w + 3], q[4 * w + 2], 0x04000c0cu);
-      c[w] = s == 255 ? 0 : lo | hi;
-    }
-  } else {
-    const float scale = as_f32(s << 23);
+  // elements of a block with scale byte s -> codes; none passes the format's largest value, and a block of scale 255 has codes 0
+  static __device__ __forceinline__ Codes encode(u32x4 v, unsigned s) {
     unsigned w0 = 0, w1 = 0;
-    if constexpr (DT == PCCL_F32) {
-      const u32x4 a = e.v[0], b = e.v[1];
-      w0 = two_down_f32<FMT, 0>(w0, as_f32(a[0]), as_f32(a[1]), scale);
-      w0 = two_down_f32<FMT, 1>(w0, as_f32(a[2]), as_f32(a[3]), scale);
-      if constexpr (CacheFormat<FMT>::kBits == 8) {
-        w1 = two_down_f32<FMT, 0>(w1, as_f32(b[0]), as_f32(b[1]), scale);
-        w1 = two_down_f32<FMT, 1>(w1, as_f32(b[2]), as_f32(b[3]), scale);
-      } else {
-        w0 = two_down_f32<FMT, 2>(w0, as_f32(b[0]), as_f32(b[1]), scale);
-        w0 = two_down_f32<FMT, 3>(w0, as_f32(b[2]), as_f32(b[3]), scale);
+    if constexpr (FMT == PCCL_CACHE_I8) {
+      float x[kElems];
+      unsigned q[kElems];
+      R::up(v, x);
+      // 64 x / scale + 1.5 * 2^23 is rounded once, to a whole number, whose low byte is the code
+      if (s >= 6 && s < 254) {  // 64 / scale is a binary32: one fused step
+        const float f = as_f32((260u - s) << 23);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) q[i] = as_u32(__builtin_fmaf(x[i], f, 12582912.0f));
+      } else {  // 1 / scale and 64 apart (exact; a subnormal product rounds to 0 either way); only here a block whose scale would be 2^128 saturates
+        const float f = as_f32(s == 254 ? 0x400000u : (254u - s) << 23);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) q[i] = as_u32(__builtin_fmaf(__builtin_amdgcn_fmed3f(x[i] * f, -127.0f / 64, 127.0f / 64), 64.0f, 12582912.0f));
       }
+      w0 = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
+      if constexpr (kElems == 8) w1 = __builtin_amdgcn_perm(q[5], q[4], 0x0c0c0400u) | __builtin_amdgcn_perm(q[7], q[6], 0x04000c0cu);
     } else {
-      const u32x4 a = e.v[0];
-      const unsigned a0 = a[0], a1 = a[1], a2 = a[2], a3 = a[3];
-      w0 = two_down<DT, FMT, 0>(w0, a0, scale);
-      w0 = two_down<DT, FMT, 1>(w0, a1, scale);
-      if constexpr (CacheFormat<FMT>::kBits == 8) {
-        w1 = two_down<DT, FMT, 0>(w1, a2, scale);
-        w1 = two_down<DT, FMT, 1>(w1, a3, scale);
+      const float scale = as_f32(s << 23);
+      const unsigned v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+      if constexpr (DT == PCCL_F32) {
+        w0 = two_down_f32<FMT, 0>(w0, as_f32(v0), as_f32(v1), scale);
+        w0 = two_down_f32<FMT, 1>(w0, as_f32(v2), as_f32(v3), scale);
       } else {
-        w0 = two_down<DT, FMT, 2>(w0, a2, scale);
-        w0 = two_down<DT, FMT, 3>(w0, a3, scale);
+        w0 = two_down<DT, FMT, 0>(w0, v0, scale);
+        w0 = two_down<DT, FMT, 1>(w0, v1, scale);
+        if constexpr (kBits == 64) {
+          w1 = two_down<DT, FMT, 0>(w1, v2, scale);
+          w1 = two_down<DT, FMT, 1>(w1, v3, scale);
+        } else {
+          w0 = two_down<DT, FMT, 2>(w0, v2, scale);
+          w0 = two_down<DT, FMT, 3>(w0, v3, scale);
+        }
       }
     }
     if (s == 255) w0 = w1 = 0;
-    if constexpr (CacheFormat<FMT>::kBits == 8) c = u32x2{w0, w1};
-    else c = w0;
+    if constexpr (kBits == 64) return u32x2{w0, w1};
+    else return w0;
   }
-  return c;
-}
+
+  static __device__ __forceinline__ Codes load_codes(const char *at, int n) {
+    if (n == kElems) return *(const typename StoredCodes<kBits>::type *)at;
+    const int bytes = (n * CacheFormat<FMT>::kBits + 7) / 8;
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kBits / 8; ++i)
+      if (i < bytes) w[i / 4] |= (unsigned)(unsigned char)at[i] << (8 * (i % 4));
+    if constexpr (kBits == 64) return u32x2{w[0], w[1]};
+    else return w[0];
+  }
+  static __device__ __forceinline__ void store_codes(char *at, int n, Codes c) {
+    if (n == kElems) {
+      typedef typename StoredCodes<kBits>::type T;
+      __builtin_nontemporal_store((T)c, (T *)at);
+    } else {
+      const int bytes = (n * CacheFormat<FMT>::kBits + 7) / 8;
+#pragma unroll
+      for (int i = 0; i < kBits / 8; ++i) {
+        unsigned w;
+        if constexpr (kBits == 64) w = c[i / 4];
+        else w = c;
+        if (i < bytes) at[i] = (char)(w >> (8 * (i % 4)));
+      }
+    }
+  }
+  // elements from `at` on, n of them there, zeros behind
+  template <bool STREAM> static __device__ __forceinline__ u32x4 load(const char *at, int n) {
+    if (n == kElems) {
+      if constexpr (STREAM) return __builtin_nontemporal_load((const typename R::pack_t *)at);
+      else return *(const typename R::pack_t *)at;
+    }
+    typename R::elem_t x[kElems];
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) x[i] = i < n ? ((const typename R::elem_t *)at)[i] : (typename R::elem_t)0;
+    return __builtin_bit_cast(u32x4, x);
+  }
+  static __device__ __forceinline__ void store(char *at, int n, u32x4 v) {
+    if (n == kElems) {
+      __builtin_nontemporal_store(v, (typename R::pack_t *)at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i)
+        if (i < n) {
+          const unsigned w = v[i * R::kBytes / 4];
+          ((typename R::elem_t *)at)[i] = (typename R::elem_t)(R::kBytes == 2 && i % 2 ? w >> 16 : w);
+        }
+    }
+  }
+};
 
 // binary32 bits of the largest magnitude of a lane's elements; magnitudes compare as whole numbers, infinities and NaN come out on top
 template <int DT>
-__device__ __forceinline__ unsigned most_of(const Eight<RowType<DT>> &e) {
+__device__ __forceinline__ unsigned most_of(u32x4 v) {
   if constexpr (DT == PCCL_F32) {
-    unsigned m = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, e.v[j][i] & 0x7fffffffu);
-    return m;
+    v &= 0x7fffffffu;
+    return max(max(v[0], v[1]), max(v[2], v[3]));
   } else {
-    const u32x4 v = e.v[0] & 0x7fff7fffu;
+    v &= 0x7fff7fffu;
     const unsigned v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
     const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v0), __builtin_bit_cast(u16x2, v1));
     const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v2), __builtin_bit_cast(u16x2, v3));
@@ -221,9 +250,13 @@ __device__ __forceinline__ unsigned most_of(const Eight<RowType<DT>> &e) {
   }
 }
 
-__device__ __forceinline__ unsigned quad_max(unsigned m) {
+// the largest of a block's 4 or 8 lanes, in each of them
+template <int LANES>
+__device__ __forceinline__ unsigned block_max(unsigned m) {
   m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
-  return max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+  m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+  if constexpr (LANES == 8) m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, true));  // row_half_mirror
+  return m;
 }
 
 // Scale byte of a block from the bits of its largest magnitude: the exponent, one more if the mantissa is beyond that of the
@@ -242,68 +275,33 @@ struct CacheArgs {
   long code_page, code_token, code_head, scale_page, scale_token, scale_head;
   long row_head;            // bytes from one head of a source or output row to the next
   int head_dim;
-  unsigned blocks;          // of a token: heads times blocks of a head
-  unsigned group;           // tokens that a wavefront has side by side (1 from 16 blocks on)
-  Divisor by_blocks, head_blocks, page_tokens, chunks;  // blocks of a token; of a head; tokens of a page; wavefronts' shares of a token
+  unsigned group;           // tokens that a wavefront has side by side
+  int parts;                // 16-byte pieces of a token that a lane has (see Place)
+  Divisor token_lanes, head_lanes, page_tokens, chunks;  // lanes that a token and a head take; tokens of a page; wavefronts' shares of a token
 };
 
-// Where a lane stands: its token among those side by side, its head's and block's offsets.
+// Where a lane stands: its token among those side by side, its head's and block's offsets.  PARTS: 16-byte pieces of a token that a
+// lane has, 64 lanes apart; 0: the token has room for others beside it.
 struct Place {
   bool on;
-  unsigned token, block;
-  int n, q;               // elements inside the head (0..8), lane of the quad
+  unsigned token;
+  int n, first;           // elements inside the head, the first of them
   long code, scale, row;  // bytes behind the token's start
 };
-template <bool ONE>  // one token at a time
-__device__ __forceinline__ Place place_of(const CacheArgs &a, unsigned chunk, int bits, int elem_bytes) {
+template <class L, int PARTS>
+__device__ __forceinline__ Place place_of(const CacheArgs &a, unsigned chunk, int part) {
   Place p;
-  const unsigned lane = threadIdx.x % kWave, at = lane / kQuad;
-  p.q = (int)(lane % kQuad);
-  p.token = ONE ? 0 : a.by_blocks.divide(at);
-  const unsigned r = ONE ? chunk * kWaveBlocks + at : at - p.token * a.blocks;
-  p.on = ONE ? r < a.blocks : p.token < a.group;
-  const unsigned head = a.head_blocks.divide(r);
-  p.block = r - head * a.head_blocks.d;
-  const int first = (int)p.block * PCCL_CACHE_BLOCK + p.q * kPerLane;
-  p.n = min(max(a.head_dim - first, 0), kPerLane);
-  p.code = (long)head * a.code_head + first * bits / 8;
-  p.scale = (long)head * a.scale_head + p.block;
-  p.row = (long)head * a.row_head + first * elem_bytes;
+  const unsigned lane = threadIdx.x % kWave;
+  p.token = PARTS ? 0 : a.token_lanes.divide(lane);
+  const unsigned r = PARTS ? (chunk * PARTS + part) * kWave + lane : lane - p.token * a.token_lanes.d;
+  p.on = PARTS ? r < a.token_lanes.d : p.token < a.group;
+  const unsigned head = a.head_lanes.divide(r);
+  p.first = (int)(r - head * a.head_lanes.d) * L::kElems;
+  p.n = min(max(a.head_dim - p.first, 0), L::kElems);
+  p.code = (long)head * a.code_head + p.first / L::kElems * (L::kBits / 8);
+  p.scale = (long)head * a.scale_head + p.first / PCCL_CACHE_BLOCK;
+  p.row = (long)head * a.row_head + p.first * L::R::kBytes;
   return p;
-}
-
-// eight elements from `at` on, n of them there, zeros behind
-template <class R>
-__device__ __forceinline__ Eight<R> load_eight(const char *at, int n) {
-  Eight<R> e;
-#pragma unroll
-  for (int j = 0; j < 8 / R::kPack; ++j) {
-    if (n == 8) {
-      e.v[j] = ((const typename R::pack_t *)at)[j];
-    } else {
-      typename R::elem_t x[R::kPack];
-#pragma unroll
-      for (int i = 0; i < R::kPack; ++i) x[i] = j * R::kPack + i < n ? ((const typename R::elem_t *)at)[j * R::kPack + i] : (typename R::elem_t)0;
-      e.v[j] = __builtin_bit_cast(u32x4, x);
-    }
-  }
-  return e;
-}
-template <class R>
-__device__ __forceinline__ void store_eight(char *at, int n, const Eight<R> &e) {
-#pragma unroll
-  for (int j = 0; j < 8 / R::kPack; ++j) {
-    if (n == 8) {
-      ((typename R::pack_t *)at)[j] = e.v[j];
-    } else {
-#pragma unroll
-      for (int i = 0; i < R::kPack; ++i)
-        if (j * R::kPack + i < n) {
-          const unsigned w = e.v[j][i * R::kBytes / 4];
-          ((typename R::elem_t *)at)[j * R::kPack + i] = (typename R::elem_t)(R::kBytes == 2 && i % 2 ? w >> 16 : w);
-        }
-    }
-  }
 }
 
 struct WriteArgs : CacheArgs {
@@ -314,50 +312,46 @@ struct WriteArgs : CacheArgs {
   unsigned tokens;  // of the launch
 };
 
-template <int DT, int FMT, int TIMES, bool ONE>
+template <int DT, int FMT, int TIMES, int PARTS, bool STREAM>
 __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) {
-  typedef RowType<DT> R;
-  typedef CacheFormat<FMT> F;
-  typedef LaneCodes<F::kBits> L;
+  typedef Lane<DT, FMT> L;
+  constexpr int kParts = PARTS ? PARTS : 1;
   const unsigned wave = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const unsigned tile = a.chunks.divide(wave), chunk = wave - tile * a.chunks.d;
   const unsigned token0 = tile * TIMES * a.group;
   if (token0 >= a.tokens) return;
-  const Place p = place_of<ONE>(a, chunk, F::kBits, R::kBytes);
   const char *src = a.srcs[blockIdx.y];
   char *codes = a.codes[blockIdx.y], *scales = a.scales[blockIdx.y];
+  Place p[kParts];
+#pragma unroll
+  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS>(a, chunk, h);
   unsigned long slot[TIMES];
-  Eight<R> e[TIMES];
+  u32x4 v[TIMES][kParts];
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    const unsigned token = token0 + t * a.group + p.token;
+    const unsigned token = token0 + t * a.group + p[0].token;
     const bool there = token < a.tokens;
     slot[t] = (unsigned long)a.slots[there ? token : 0];  // (no branch around the load: all of them go out together)
     if (!there) slot[t] = ~0ul;
   }
 #pragma unroll
   for (int t = 0; t < TIMES; ++t)
-    if (slot[t] < a.n_slots && p.on) e[t] = load_eight<R>(src + (unsigned long)(token0 + t * a.group + p.token) * a.src_token + p.row, p.n);
+#pragma unroll
+    for (int h = 0; h < kParts; ++h)
+      if (slot[t] < a.n_slots && p[h].on)
+        v[t][h] = L::template load<STREAM>(src + (unsigned long)(token0 + t * a.group + p[0].token) * a.src_token + p[h].row, p[h].n);
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    if (slot[t] >= a.n_slots || !p.on) continue;  // whole quads
-    const unsigned s = scale_of<F>(quad_max(most_of<DT>(e[t])));
-    const typename L::type c = encode<DT, FMT>(e[t], s);
     const unsigned page = a.page_tokens.divide((unsigned)slot[t]), token = (unsigned)slot[t] - page * a.page_tokens.d;
-    char *to = codes + ((unsigned long)page * a.code_page + (unsigned long)token * a.code_token) + p.code;
-    if (p.n == 8) {
-      *(typename L::any *)to = c;
-    } else {
-      const int bytes = (p.n * F::kBits + 7) / 8;
+    char *to = codes + ((unsigned long)page * a.code_page + (unsigned long)token * a.code_token);
+    char *scale_to = scales + ((unsigned long)page * a.scale_page + (unsigned long)token * a.scale_token);
 #pragma unroll
-      for (int i = 0; i < F::kBits; ++i) {
-        unsigned w;
-        if constexpr (F::kBits == 8) w = c[i / 4];
-        else w = c;
-        if (i < bytes) to[i] = (char)(w >> (8 * (i % 4)));
-      }
+    for (int h = 0; h < kParts; ++h) {
+      if (slot[t] >= a.n_slots || !p[h].on) continue;  // whole blocks
+      const unsigned s = scale_of<CacheFormat<FMT>>(block_max<L::kBlockLanes>(most_of<DT>(v[t][h])));
+      L::store_codes(to + p[h].code, p[h].n, L::encode(v[t][h], s));
+      if (p[h].first % PCCL_CACHE_BLOCK == 0) scale_to[p[h].scale] = (char)s;
     }
-    if (p.q == 0) scales[((unsigned long)page * a.scale_page + (unsigned long)token * a.scale_token) + p.scale] = (char)s;
   }
 }
 
@@ -371,56 +365,60 @@ struct ReadArgs : CacheArgs {
   int seq0;
 };
 
-template <int DT, int FMT, int TIMES, bool ONE>
+template <int DT, int FMT, int TIMES, int PARTS>
 __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
-  typedef RowType<DT> R;
-  typedef CacheFormat<FMT> F;
-  typedef LaneCodes<F::kBits> L;
+  typedef Lane<DT, FMT> L;
+  constexpr int kParts = PARTS ? PARTS : 1;
   const long seq = a.seq0 + (long)blockIdx.y;
   const unsigned wave = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const unsigned tile = a.chunks.divide(wave), chunk = wave - tile * a.chunks.d;
   const unsigned long token0 = a.token0 + (unsigned long)tile * TIMES * a.group;
-  long length = a.lengths[seq];
-  if (length > a.max_len) length = a.max_len;
-  if ((long)token0 >= length) return;
-  const Place p = place_of<ONE>(a, chunk, F::kBits, R::kBytes);
-  const char *codes = a.codes[blockIdx.z], *scales = a.scales[blockIdx.z];
-  char *out = a.outs[blockIdx.z];
-  const long first_row = a.row_start ? a.row_start[seq] : seq * a.max_len;
+  if ((long)token0 >= a.max_len) return;
+  Place p[kParts];
+#pragma unroll
+  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS>(a, chunk, h);
+  // Table entries, length and first row are asked for together (an entry that is not the sequence's is inside the table all the
+  // same): what a wavefront waits for is one chain of two loads.
   const int *table = a.page_table + seq * a.table_stride;
   unsigned long page[TIMES];
-  typename L::type c[TIMES];
-  unsigned s[TIMES];
+  bool named[TIMES];
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    const unsigned pos = (unsigned)token0 + t * a.group + p.token, entry = a.page_tokens.divide(pos);
-    const bool named = (long)pos < length && (long)entry < a.table_stride && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows;
-    page[t] = (unsigned long)(long)table[named ? entry : 0];  // (no branch around the load: all of them go out together)
-    if (!named) page[t] = ~0ul;
+    const unsigned pos = (unsigned)token0 + t * a.group + p[0].token, entry = a.page_tokens.divide(pos);
+    named[t] = (long)entry < a.table_stride;
+    page[t] = (unsigned long)(long)table[named[t] ? entry : 0];
+  }
+  long length = a.lengths[seq];
+  const long first_row = a.row_start ? a.row_start[seq] : seq * a.max_len;
+  const char *codes = a.codes[blockIdx.z], *scales = a.scales[blockIdx.z];
+  char *out = a.outs[blockIdx.z];
+  if (length > a.max_len) length = a.max_len;
+  typename L::Codes c[TIMES][kParts];
+  unsigned s[TIMES][kParts];
+#pragma unroll
+  for (int t = 0; t < TIMES; ++t) {
+    const unsigned pos = (unsigned)token0 + t * a.group + p[0].token;
+    named[t] = named[t] && (long)pos < length && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows && page[t] < (unsigned long)a.n_pages;
   }
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    if (page[t] >= (unsigned long)a.n_pages || !p.on) continue;
-    const unsigned pos = (unsigned)token0 + t * a.group + p.token, token = pos - a.page_tokens.divide(pos) * a.page_tokens.d;
-    const char *from = codes + (page[t] * a.code_page + (unsigned long)token * a.code_token) + p.code;
-    s[t] = (unsigned char)(scales + (page[t] * a.scale_page + (unsigned long)token * a.scale_token))[p.scale];
-    if (p.n == 8) {
-      c[t] = *(const typename L::any *)from;
-    } else {
-      const int bytes = (p.n * F::kBits + 7) / 8;
-      unsigned w[2] = {0, 0};
+    const unsigned pos = (unsigned)token0 + t * a.group + p[0].token, token = pos - a.page_tokens.divide(pos) * a.page_tokens.d;
+    const char *from = codes + (page[t] * a.code_page + (unsigned long)token * a.code_token);
+    const char *scale_from = scales + (page[t] * a.scale_page + (unsigned long)token * a.scale_token);
 #pragma unroll
-      for (int i = 0; i < F::kBits; ++i)
-        if (i < bytes) w[i / 4] |= (unsigned)(unsigned char)from[i] << (8 * (i % 4));
-      if constexpr (F::kBits == 8) c[t] = u32x2{w[0], w[1]};
-      else c[t] = w[0];
+    for (int h = 0; h < kParts; ++h) {
+      if (!named[t] || !p[h].on) continue;
+      s[t][h] = (unsigned char)scale_from[p[h].scale];
+      c[t][h] = L::load_codes(from + p[h].code, p[h].n);
     }
   }
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
-    if (page[t] >= (unsigned long)a.n_pages || !p.on) continue;
-    const unsigned pos = (unsigned)token0 + t * a.group + p.token;
-    store_eight<R>(out + (unsigned long)(first_row + pos) * a.out_token + p.row, p.n, decode<DT, FMT>(c[t], s[t]));
+    const unsigned pos = (unsigned)token0 + t * a.group + p[0].token;
+    char *to = out + (unsigned long)(first_row + pos) * a.out_token;
+#pragma unroll
+    for (int h = 0; h < kParts; ++h)
+      if (named[t] && p[h].on) L::store(to + p[h].row, p[h].n, L::decode(c[t][h], s[t][h]));
   }
 }
 
@@ -444,7 +442,7 @@ bool apart(const long (&count)[3], const long (&stride)[3], long bytes) {
   return true;
 }
 
-int check_cache(const pccl_cache_desc *c, int dtype, const void *const *tensors, const char *what, CacheArgs *a) {
+int check_cache(const pccl_cache_desc *c, int dtype, const void *const *tensors, const char *what, bool whole_blocks, CacheArgs *a) {
   if (!c) return fail(PCCL_ERR_INVALID_ARG, "cache: description is null");
   if (c->format < PCCL_CACHE_F8E4M3 || c->format > PCCL_CACHE_F4E2M1) return fail(PCCL_ERR_UNSUPPORTED, "unknown cache format %d", c->format);
   if (dtype != PCCL_F32 && dtype != PCCL_BF16 && dtype != PCCL_F16) return fail(PCCL_ERR_UNSUPPORTED, "cache: rows of dtype code %d", dtype);
@@ -479,12 +477,15 @@ int check_cache(const pccl_cache_desc *c, int dtype, const void *const *tensors,
   a->scale_token = c->scale_token;
   a->scale_head = c->scale_head;
   a->head_dim = c->head_dim;
-  a->blocks = (unsigned)c->heads * (unsigned)blocks;  // at most 2^27
-  a->group = std::max(1u, kWaveBlocks / a->blocks);
-  a->by_blocks.set(a->blocks);
-  a->head_blocks.set((unsigned)blocks);
+  // lanes of a head: as many as its elements fill, when writing as many as its blocks have (at most 2^14, of a token 2^30)
+  const int elems = 16 / es, head_lanes = whole_blocks ? blocks * (PCCL_CACHE_BLOCK / elems) : (c->head_dim + elems - 1) / elems;
+  const unsigned token_lanes = (unsigned)c->heads * (unsigned)head_lanes;
+  a->group = std::max(1u, kWave / token_lanes);
+  a->token_lanes.set(token_lanes);
+  a->head_lanes.set((unsigned)head_lanes);
   a->page_tokens.set((unsigned)c->page_tokens);
-  a->chunks.set(a->group > 1 ? 1 : (a->blocks + kWaveBlocks - 1) / kWaveBlocks);
+  a->parts = a->group > 1 ? 0 : token_lanes > kWave ? 2 : 1;
+  a->chunks.set(a->parts < 2 ? 1 : (token_lanes + 2 * kWave - 1) / (2 * kWave));
   return PCCL_OK;
 }
 
@@ -503,10 +504,14 @@ void with_types(int dtype, int format, F &&f) {
   else of_format(std::integral_constant<int, PCCL_F16>{});
 }
 
-constexpr int kTimes = 4;  // groups of tokens that a wavefront has in flight where there are enough of them
+#ifndef WT
+#define WT 2
+#define RT 4
+#endif
+constexpr int kWriteTimes = WT, kReadTimes = RT;  // groups of tokens that a wavefront has in flight where there are enough of them
 
-// whether n wavefronts' worth of tokens give every compute unit eight workgroups of kTimes groups a wavefront
-bool many(long n) { return n >= (long)pccl_host::compute_units() * 8 * kWaves * kTimes; }
+// whether n wavefronts' worth of tokens, `times` of them to a wavefront, give every compute unit eight workgroups
+bool many(long n, int times) { return n >= (long)pccl_host::compute_units() * 8 * kWaves * times; }
 
 // Tokens of a launch: wavefronts stay below 2^26 (a grid times its lanes must fit 32 bits) and below what Divisor divides.
 long launch_tokens(const CacheArgs &a) { return std::max(1l, (1l << 26) / a.chunks.d); }
@@ -517,13 +522,16 @@ unsigned workgroups(const CacheArgs &a, long tokens, int times) {
   return (unsigned)((tiles * a.chunks.d + kWaves - 1) / kWaves);
 }
 
-// Calls f(times, one token at a time) with both as constants.
-template <class F>
-void with_shape(bool four, bool one, F &&f) {
-  typedef std::integral_constant<int, kTimes> Four;
-  typedef std::integral_constant<int, 1> Once;
-  if (four) one ? f(Four{}, std::true_type{}) : f(Four{}, std::false_type{});
-  else one ? f(Once{}, std::true_type{}) : f(Once{}, std::false_type{});
+// Calls f(times, parts) with both as constants.
+template <int TIMES, class F>
+void with_shape(bool several, int parts, F &&f) {
+  auto of_parts = [&](auto times) {
+    if (parts == 0) f(times, std::integral_constant<int, 0>{});
+    else if (parts == 1) f(times, std::integral_constant<int, 1>{});
+    else f(times, std::integral_constant<int, 2>{});
+  };
+  if (several) of_parts(std::integral_constant<int, TIMES>{});
+  else of_parts(std::integral_constant<int, 1>{});
 }
 
 int launched(const char *what) {
@@ -537,7 +545,7 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
                                     const long *slots, long tokens, void *stream) {
   pccl_host::clear_error();
   WriteArgs a;
-  int rc = check_cache(c, dtype, srcs, "source", &a);
+  int rc = check_cache(c, dtype, srcs, "source", true, &a);
   if (rc != PCCL_OK) return rc;
   if (tokens < 0 || tokens > 0x7fffffffl) return fail(PCCL_ERR_INVALID_ARG, "tokens %ld outside [0, 2^31)", tokens);
   if (src_token_stride < 0 || src_head_stride < 0)
@@ -553,17 +561,19 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
   a.src_token = src_token_stride * es;
   a.row_head = src_head_stride * es;
   a.n_slots = (unsigned long)(c->n_pages * c->page_tokens);
+  const bool stream_in = (long)c->heads * c->head_dim * es * tokens * c->n_tensors >= (48l << 20);
   const long most = launch_tokens(a);
   for (long lo = 0; lo < tokens; lo += most) {
     const long n = std::min(most, tokens - lo);
     for (int k = 0; k < c->n_tensors; ++k) a.srcs[k] = (const char *)srcs[k] + lo * a.src_token;
     a.slots = slots + lo;
     a.tokens = (unsigned)n;
-    const bool four = many((n + a.group - 1) / a.group * a.chunks.d * c->n_tensors);
     with_types(dtype, c->format, [&](auto t, auto f) {
-      with_shape(four, a.group == 1, [&](auto times, auto one) {
-        hipLaunchKernelGGL((cache_write_kernel<decltype(t)::value, decltype(f)::value, decltype(times)::value, decltype(one)::value>),
-                           dim3(workgroups(a, n, decltype(times)::value), c->n_tensors), dim3(kBlock), 0, (hipStream_t)stream, a);
+      with_shape<kWriteTimes>(many((n + a.group - 1) / a.group * a.chunks.d * c->n_tensors, kWriteTimes), a.parts, [&](auto times, auto parts) {
+        constexpr int DT = decltype(t)::value, FMT = decltype(f)::value, TIMES = decltype(times)::value, PARTS = decltype(parts)::value;
+        const dim3 grid(workgroups(a, n, TIMES), c->n_tensors);
+        if (stream_in) hipLaunchKernelGGL((cache_write_kernel<DT, FMT, TIMES, PARTS, true>), grid, dim3(kBlock), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((cache_write_kernel<DT, FMT, TIMES, PARTS, false>), grid, dim3(kBlock), 0, (hipStream_t)stream, a);
       });
     });
     rc = launched("cache_write");
@@ -577,7 +587,7 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
                                    int n_seq, long max_len, void *stream) {
   pccl_host::clear_error();
   ReadArgs a;
-  int rc = check_cache(c, dtype, (const void *const *)outs, "output", &a);
+  int rc = check_cache(c, dtype, (const void *const *)outs, "output", false, &a);
   if (rc != PCCL_OK) return rc;
   if (n_seq < 0) return fail(PCCL_ERR_INVALID_ARG, "n_seq %d < 0", n_seq);
   if (max_len < 0 || max_len > 0x7fffffffl) return fail(PCCL_ERR_INVALID_ARG, "max_len %ld outside [0, 2^31)", max_len);
@@ -612,11 +622,11 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
     for (long lo = 0; lo < max_len; lo += most) {
       a.token0 = (unsigned)lo;
       const long n = std::min(most, max_len - lo);
-      const bool four = many((n + a.group - 1) / a.group * a.chunks.d * seqs * c->n_tensors);
       with_types(dtype, c->format, [&](auto t, auto f) {
-        with_shape(four, a.group == 1, [&](auto times, auto one) {
-          hipLaunchKernelGGL((cache_read_kernel<decltype(t)::value, decltype(f)::value, decltype(times)::value, decltype(one)::value>),
-                             dim3(workgroups(a, n, decltype(times)::value), seqs, c->n_tensors), dim3(kBlock), 0, (hipStream_t)stream, a);
+        with_shape<kReadTimes>(many((n + a.group - 1) / a.group * a.chunks.d * seqs * c->n_tensors, kReadTimes), a.parts, [&](auto times, auto parts) {
+          constexpr int DT = decltype(t)::value, FMT = decltype(f)::value, TIMES = decltype(times)::value, PARTS = decltype(parts)::value;
+          hipLaunchKernelGGL((cache_read_kernel<DT, FMT, TIMES, PARTS>), dim3(workgroups(a, n, TIMES), seqs, c->n_tensors), dim3(kBlock), 0,
+                             (hipStream_t)stream, a);
         });
       });
       rc = launched("cache_read");
