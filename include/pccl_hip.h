@@ -246,7 +246,7 @@ enum pccl_cache_format { PCCL_CACHE_F8E4M3 = 0, PCCL_CACHE_F8E5M2 = 1, PCCL_CACH
 /* n_tensors caches of one shape (keys and values, or those of several layers).  Codes of page p, token t of the page and head
  * h start at codes + p * code_page + t * code_token + h * code_head (bytes, ceil(head_dim * bits / 8) of them), its scales at
  * scales + p * scale_page + t * scale_token + h * scale_head (ceil(head_dim / 32) bytes).  Any order of the three that keeps
- * heads apart; any alignment. */
+ * heads apart; any alignment.  Strides of pages and tokens, a source's or output's of tokens as well, are below 4 GiB. */
 typedef struct pccl_cache_desc {
   int format;                /* enum pccl_cache_format              */
   int n_tensors;             /* 1..8                                */
