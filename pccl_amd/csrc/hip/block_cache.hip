@@ -19,6 +19,8 @@ namespace pccl_dev {
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef unsigned int u32_a1 __attribute__((aligned(1)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+typedef unsigned int u32_a2 __attribute__((aligned(2)));
 typedef unsigned short u16_a1 __attribute__((aligned(1)));
 
 constexpr int kWaves = kBlock / kWave;
@@ -184,9 +186,22 @@ struct Lane {
     else return w0;
   }
 
-  static __device__ __forceinline__ Codes load_codes(const char *at, int n) {
-    if (n == kElems) return *(const typename StoredCodes<kBits>::type *)at;
+  // The last piece of a head may be short (n elements of kElems, none for a lane behind it).  It is loaded as the whole piece that ends
+  // with the head and shifted down, where the head is long enough for that (`long_head`), and stored as pieces of 8, 4, 2 and 1
+  // bytes: element by element the one short piece of an odd head cost as much as all the others together.
+  static __device__ __forceinline__ Codes load_codes(const char *at, int n, bool long_head) {
+    typedef typename StoredCodes<kBits>::type T;
+    if (n == kElems) return *(const T *)at;
     const int bytes = (n * CacheFormat<FMT>::kBits + 7) / 8;
+    if (long_head) {
+      const Codes c = *(const T *)(at + bytes - kBits / 8);
+      if constexpr (kBits == 64) {
+        const unsigned long w = __builtin_bit_cast(unsigned long, c) >> (8 * (8 - bytes));
+        return __builtin_bit_cast(u32x2, w);
+      } else {
+        return c >> (8 * (kBits / 8 - bytes));
+      }
+    }
     unsigned w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < kBits / 8; ++i)
@@ -195,25 +210,44 @@ struct Lane {
     else return w[0];
   }
   static __device__ __forceinline__ void store_codes(char *at, int n, Codes c) {
-    if (n == kElems) {
+    const int bytes = (n * CacheFormat<FMT>::kBits + 7) / 8;
+    if (bytes == kBits / 8) {  // (with 4-bit codes also where the last code's half of the byte is empty)
       typedef typename StoredCodes<kBits>::type T;
       __builtin_nontemporal_store((T)c, (T *)at);
     } else {
-      const int bytes = (n * CacheFormat<FMT>::kBits + 7) / 8;
-#pragma unroll
-      for (int i = 0; i < kBits / 8; ++i) {
-        unsigned w;
-        if constexpr (kBits == 64) w = c[i / 4];
-        else w = c;
-        if (i < bytes) at[i] = (char)(w >> (8 * (i % 4)));
+      unsigned w;  // what is left to store
+      if constexpr (kBits == 64) w = bytes & 4 ? c[1] : c[0];
+      else w = c;
+      if constexpr (kBits == 64) {
+        if (bytes & 4) {
+          const unsigned first = c[0];
+          *(u32_a1 *)at = first;
+          at += 4;
+        }
       }
+      if (bytes & 2) {
+        *(u16_a1 *)at = (unsigned short)w;
+        at += 2;
+        w >>= 16;
+      }
+      if (bytes & 1) *at = (char)w;
     }
   }
   // elements from `at` on, n of them there, zeros behind
-  template <bool STREAM> static __device__ __forceinline__ u32x4 load(const char *at, int n) {
+  template <bool STREAM> static __device__ __forceinline__ u32x4 load(const char *at, int n, bool long_head) {
+    typedef typename R::pack_t T;
     if (n == kElems) {
-      if constexpr (STREAM) return __builtin_nontemporal_load((const typename R::pack_t *)at);
-      else return *(const typename R::pack_t *)at;
+      if constexpr (STREAM) return __builtin_nontemporal_load((const T *)at);
+      else return *(const T *)at;
+    }
+    if (n > 0 && long_head) {
+      u32x4 v = *(const T *)(at + (n - kElems) * R::kBytes);
+      const int skip = (kElems - n) * R::kBytes;  // bytes to shift down by: 8, 4 and 2 of them
+      if (skip & 8) v = u32x4{v[2], v[3], 0, 0};
+      if (skip & 4) v = u32x4{v[1], v[2], v[3], 0};
+      if (R::kBytes == 2 && (skip & 2))
+        v = u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], 2), __builtin_amdgcn_alignbyte(v[2], v[1], 2), __builtin_amdgcn_alignbyte(v[3], v[2], 2), v[3] >> 16};
+      return v;
     }
     typename R::elem_t x[kElems];
 #pragma unroll
@@ -224,12 +258,19 @@ struct Lane {
     if (n == kElems) {
       __builtin_nontemporal_store(v, (typename R::pack_t *)at);
     } else {
-#pragma unroll
-      for (int i = 0; i < kElems; ++i)
-        if (i < n) {
-          const unsigned w = v[i * R::kBytes / 4];
-          ((typename R::elem_t *)at)[i] = (typename R::elem_t)(R::kBytes == 2 && i % 2 ? w >> 16 : w);
-        }
+      const int bytes = n * R::kBytes;
+      if (bytes & 8) {
+        *(u32x2_a2 *)at = u32x2{v[0], v[1]};
+        at += 8;
+      }
+      unsigned w = bytes & 8 ? v[2] : v[0];
+      const unsigned after = bytes & 8 ? v[3] : v[1];
+      if (bytes & 4) {
+        *(u32_a2 *)at = w;
+        at += 4;
+        w = after;
+      }
+      if (R::kBytes == 2 && (bytes & 2)) *(unsigned short *)at = (unsigned short)w;
     }
   }
 };
@@ -348,6 +389,7 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
     slot[t] = (unsigned long)a.slots[there ? token : 0];  // (no branch around the load: all of them go out together)
     if (!there) slot[t] = ~0ul;
   }
+  const bool long_head = a.head_dim >= L::kElems;
   auto work = [&](auto whole) {
     constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
@@ -355,7 +397,7 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
 #pragma unroll
       for (int h = 0; h < kParts; ++h)
         if (kWhole || (slot[t] < a.n_slots && p[h].on))
-          v[t][h] = L::template load<STREAM>(src + times(token0 + t * a.group + p[0].token, a.src_token) + p[h].row, kWhole ? L::kElems : p[h].n);
+          v[t][h] = L::template load<STREAM>(src + times(token0 + t * a.group + p[0].token, a.src_token) + p[h].row, kWhole ? L::kElems : p[h].n, long_head);
 #pragma unroll
     for (int t = 0; t < TIMES; ++t) {
       const unsigned page = a.page_tokens.divide((unsigned)slot[t]), token = (unsigned)slot[t] - page * a.page_tokens.d;
@@ -424,6 +466,7 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
     const unsigned pos = (unsigned)token0 + t * a.group + p[0].token;
     named[t] = named[t] && (long)pos < length && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows && page[t] < (unsigned long)a.n_pages;
   }
+  const bool long_head = a.head_dim >= L::kElems;
   auto work = [&](auto whole) {
     constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
@@ -435,7 +478,7 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
       for (int h = 0; h < kParts; ++h) {
         if (!kWhole && (!named[t] || !p[h].on)) continue;
         s[t][h] = (unsigned char)scale_from[p[h].scale];
-        c[t][h] = L::load_codes(from + p[h].code, kWhole ? L::kElems : p[h].n);
+        c[t][h] = L::load_codes(from + p[h].code, kWhole ? L::kElems : p[h].n, long_head);
       }
     }
 #pragma unroll
