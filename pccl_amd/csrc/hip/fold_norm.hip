@@ -15,15 +15,10 @@ namespace {
 // Rows of a launch: a grid times its lanes must fit 32 bits, 2^22 - 1 workgroups of 1024.
 constexpr unsigned kLaunchRows = 1u << 21;
 
-// Teams of the smallest shape that holds the width: a wavefront up to 512 elements (no barrier in its sums), a
-// workgroup beyond.
+// A wavefront up to 512 elements (no barrier in its sums), beyond a workgroup of as many wavefronts as the width fills.
 NormShape shape_of(long width) {
-  if (width <= 512) return {64, 8};
-  if (width <= 1024) return {128, 8};
-  if (width <= 2048) return {256, 8};
-  if (width <= 4096) return {512, 8};
-  if (width <= 8192) return {1024, 8};
-  return {1024, 16};
+  const int elems = width <= 8192 ? 8 : 16;
+  return {(int)((width + elems * kWave - 1) / (elems * kWave)) * kWave, elems};
 }
 
 bool row_dtype(int dtype) { return dtype == PCCL_F32 || dtype == PCCL_BF16 || dtype == PCCL_F16; }
@@ -129,20 +124,18 @@ int launched(hipError_t e, const char *what) {
 
 // How the backward pass cuts the rows (see BackwardArgs).
 struct Cut {
-  unsigned groups, strips, strip_rows, n_strips, n_teams;
+  unsigned groups, strips, n_strips, n_teams;
 };
 
 // Teams that fill the chip: enough for several wavefronts on every SIMD, few enough that writing and joining their sums
 // (4 rows of binary32 a team) stays small beside the rows themselves.
 Cut cut_of(long rows, long width, long gate_rows) {
   const NormShape n = shape_of(width);
-  const long most = (long)pccl_host::compute_units() * (1024 / n.lanes);
+  const long most = (long)pccl_host::compute_units() * (kMostLanes / n.lanes);
   const long per = gate_rows >= 1 ? std::min(gate_rows, std::max(1l, rows)) : std::max(1l, rows);
   Cut c;
   c.groups = (unsigned)std::max(1l, gate_row_count(rows, per));
-  long strips = std::max(1l, std::min(per, most / (long)c.groups));
-  c.strip_rows = (unsigned)((per + strips - 1) / strips);
-  c.strips = (unsigned)((per + c.strip_rows - 1) / c.strip_rows);
+  c.strips = (unsigned)std::max(1l, std::min(per, most / (long)c.groups));
   c.n_strips = c.groups * c.strips;
   c.n_teams = (unsigned)std::min<long>(c.n_strips, most);
   return c;
@@ -181,11 +174,14 @@ extern "C" int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream) {
   for (int j = 0; j < d->n_out; ++j) a.outs[j] = (char *)d->outs[j];
   a.out_bytes = d->out_stride * c.es;
   const NormShape n = shape_of(d->width);
+  // many inputs beyond the Infinity Cache are read non-temporally (8 -> 8 bf16 at 2048 x 8192 122 -> 120 us, 8 -> 1 at 4096 x 4096 67 -> 64;
+  // one or two lose: 1 -> 1 at 16384 x 8192 178 -> 184, and so does what is in that cache: f32 2 -> 2 at 4096 x 2048 38 -> 45)
+  const bool stream_in = (d->n_in + d->n_out + 2) * d->rows * d->width * c.es > (256l << 20);
   for (long lo = 0; lo < d->rows; lo += kLaunchRows) {
     a.row0 = (unsigned)lo;
     a.rows = (unsigned)std::min<long>(d->rows, lo + kLaunchRows);
     rc = launched(with_types(d->dtype, d->param_dtype, [&](auto t, auto p) {
-      return launch_fold_norm<decltype(t)::value, decltype(p)::value>(n, (hipStream_t)stream, a);
+      return launch_fold_norm<decltype(t)::value, decltype(p)::value>(n, stream_in, (hipStream_t)stream, a);
     }), "fold_norm");
     if (rc != PCCL_OK) return rc;
   }
@@ -263,7 +259,6 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   a.n_grad_in = g->n_grad_in;
   a.grad_in_bytes = g->grad_in_stride * c.es;
   a.n_strips = cut.n_strips;
-  a.strip_rows = cut.strip_rows;
   a.strips = cut.strips;
   a.n_teams = cut.n_teams;
   a.sums = (float *)g->workspace;
@@ -271,9 +266,11 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   a.grad_gate = d->rows ? (char *)g->grad_gate : nullptr;  // (no rows: no gate row either)
   a.grad_gate_bytes = g->grad_gate_stride * c.ps;
   for (int k = 0; k < 4; ++k) a.want_sums[k] = to[k] != nullptr;
+  // beyond the Infinity Cache (bf16 16384 x 8192 306 -> 281 us, 32768 x 1024 88 -> 83; inside: 8192 x 2048 with a gate a row 84.5 -> 86)
+  const bool stream_in = (4 + g->n_grad_in) * d->rows * d->width * c.es > (256l << 20);
   const bool bias = to[1] || to[3] || (g->grad_gate && d->post_bias);
   rc = launched(with_types(d->dtype, d->param_dtype, [&](auto t, auto p) {
-    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape_of(d->width), bias, (hipStream_t)stream, a);
+    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape_of(d->width), bias, stream_in, (hipStream_t)stream, a);
   }), "fold_norm_backward");
   if (rc != PCCL_OK || !need) return rc;
 
@@ -286,7 +283,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
     if (to[k]) j.listed[j.n_listed++] = k;
   }
   j.width = (int)d->width;
-  j.n_teams = cut.n_teams;
+  j.n_partial = shape_of(d->width).workgroups(cut.n_teams);
   j.strips = cut.strips;
   j.grad_gate = a.grad_gate;
   j.grad_gate_bytes = a.grad_gate_bytes;

@@ -1,9 +1,10 @@
 // fold_norm_device.h -- device code shared by the forward and backward kernels of the norms around a
 // block: how a row lies over the lanes of a team, loads and stores of a lane's share, sums over a team.
 //
-// A row of `width` elements is worked on by a team of LANES lanes (one wavefront, or one workgroup) and stays in
-// their registers from the first load to the last store: E elements a lane, as E / kPack packs of 16 bytes;
-// pack j of lane l is pack j * LANES + l of the row, so that an instruction of a wavefront covers 1 KiB.
+// A row of `width` elements is worked on by a team of lanes (TEAM false: one wavefront, four of them to a workgroup; TEAM true: a
+// workgroup of as many wavefronts as the width needs) and stays in their registers from the first load to the last
+// store: E elements a lane, as E / kPack packs of 16 bytes; pack j of lane l is pack j * lanes + l of the row, so that an
+// instruction of a wavefront covers 1 KiB.
 // Where the width is no multiple of a pack, the row's last pack is moved back to end with the row and the `lo`
 // elements at its front, which the pack before it holds as well, are masked: left out of sums, not stored.
 // (So every load is one 16-byte load inside the row at any width of at least a pack and any element alignment;
@@ -92,29 +93,30 @@ template <> struct RowType<PCCL_F16> {
 };
 
 // One lane's share of a row: E elements of the packs of type R::kPack.
-template <class R, int LANES, int E>
+template <class R, bool TEAM, int E>
 struct Share {
   static constexpr int kPacks = E / R::kPack;
-  static constexpr bool kMayBeNarrow = LANES == kWave && E == 8;  // the shape that rows of less than a pack are given to
+  static constexpr bool kMayBeNarrow = !TEAM;  // rows of less than a pack are given to one wavefront
   int off[kPacks];  // where pack j starts in the row (below 0 in a narrow row: its first elements are masked)
   int lo[kPacks];   // elements at its front that are not this lane's; R::kPack or more: no pack
   bool narrow;      // the row is shorter than a pack
   bool ragged;      // some element of some lane is masked
 
-  __device__ __forceinline__ Share(int lane, int width) {
+  __device__ __forceinline__ Share(int lane, int lanes, int width) {
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
-      const int first = (j * LANES + lane) * R::kPack;
+      const int first = (j * lanes + lane) * R::kPack;
       off[j] = first < width - R::kPack ? first : width - R::kPack;
       lo[j] = first - off[j];
     }
     narrow = kMayBeNarrow && width < R::kPack;
-    ragged = width != LANES * E;
+    ragged = width != lanes * E;
   }
   __device__ __forceinline__ bool has(int j) const { return lo[j] < R::kPack; }
 
   // this lane's packs of the row at `row` (wave-uniform), zeros where it has none
-  __device__ __forceinline__ void load(const char *row, u32x4 (&v)[kPacks]) const {
+  // (STREAM: non-temporal)
+  template <bool STREAM = false> __device__ __forceinline__ void load(const char *row, u32x4 (&v)[kPacks]) const {
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       v[j] = u32x4{0, 0, 0, 0};
@@ -125,16 +127,19 @@ struct Share {
           for (int i = 0; i < R::kPack; ++i) e[i] = i >= lo[j] ? ((const typename R::elem_t *)row)[off[j] + i] : (typename R::elem_t)0;
           v[j] = __builtin_bit_cast(u32x4, e);
         } else {
-          v[j] = *(const typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes);
+          const typename R::pack_t *at = (const typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes);
+          if constexpr (STREAM) v[j] = __builtin_nontemporal_load(at);
+          else v[j] = *at;
         }
       }
     }
   }
+  // Rows are stored non-temporally at every size (forward f32 2 -> 2 at 4096 x 2048 45 -> 38 us, bf16 8 -> 8 at 2048 x 8192 129 -> 122).
   __device__ __forceinline__ void store(char *row, const float (&x)[E]) const {
 #pragma unroll
     for (int j = 0; j < kPacks; ++j) {
       if (lo[j] == 0) {
-        *(typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes) = R::down(x + j * R::kPack);
+        __builtin_nontemporal_store(R::down(x + j * R::kPack), (typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes));
       } else if (has(j)) {
 #pragma unroll
         for (int i = 0; i < R::kPack; ++i)
@@ -162,14 +167,14 @@ struct Share {
 };
 
 // One lane's share of a parameter row (weight, bias, gate): elements of the rows' type or binary32.
-template <class R, bool PF32, int LANES, int E>
+template <class R, bool PF32, bool TEAM, int E>
 struct ParamShare {
   static constexpr int kPacks = E / R::kPack;
   static constexpr bool kWide = PF32 && R::kBytes == 2;  // a pack's parameters are two 16-byte loads
   static constexpr int kWords = kWide ? 2 * kPacks : kPacks;
   u32x4 v[kWords];
 
-  __device__ __forceinline__ void load(const Share<R, LANES, E> &s, const char *row) {
+  __device__ __forceinline__ void load(const Share<R, TEAM, E> &s, const char *row) {
     if constexpr (!kWide) {
       s.load(row, v);
     } else {
@@ -194,7 +199,7 @@ struct ParamShare {
   }
   __device__ __forceinline__ void up(float (&x)[E]) const {
     if constexpr (!kWide) {
-      Share<R, LANES, E>::up(v, x);
+      Share<R, TEAM, E>::up(v, x);
     } else {
 #pragma unroll
       for (int w = 0; w < kWords; ++w)
@@ -205,14 +210,14 @@ struct ParamShare {
 };
 
 // y = the left fold of this lane's share of n rows.  AT_ONCE inputs are in flight together.
-template <class R, int LANES, int E, int AT_ONCE, class Ins>
-__device__ __forceinline__ void fold_rows(const Share<R, LANES, E> &s, const Ins &ins, int n, long at, float (&y)[E]) {
+template <bool STREAM, int AT_ONCE, class R, bool TEAM, int E, class Ins>
+__device__ __forceinline__ void fold_rows(const Share<R, TEAM, E> &s, const Ins &ins, int n, long at, float (&y)[E]) {
   constexpr int kPacks = E / R::kPack;
   for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
     u32x4 v[AT_ONCE][kPacks];
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k)
-      if (k == 0 || k0 + k < n) s.load(ins[k0 + k] + at, v[k]);
+      if (k == 0 || k0 + k < n) s.template load<STREAM>(ins[k0 + k] + at, v[k]);
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
       if (k == 0 || k0 + k < n) {
@@ -253,17 +258,15 @@ __device__ __forceinline__ float of_lane(float x, int lane) { return as_f32((uns
 // the sixteen lanes of a row read one each and add them as above (reading all of them into every lane cost 64 registers).
 // `turn` alternates between two sets of LDS words, so that one barrier a sum is enough: a wavefront writes a set again only
 // after the barrier of the sum in between, which every reader of the set has reached.
-constexpr int kSumsAtOnce = 4;
-template <int LANES>
+constexpr int kSumsAtOnce = 4, kMostWaves = 16;
+template <bool TEAM>
 struct TeamSums {
-  static constexpr int kWaves = LANES / kWave;
-  static_assert(kWaves <= 16, "one lane of a row per wavefront");
-  float (*words)[kWaves][kSumsAtOnce];  // [2]
-  int turn;
+  float (*words)[TEAM ? kMostWaves : 1][kSumsAtOnce];  // [2]
+  int waves, turn;  // a row of 16 lanes has one for each wavefront
 
   template <int N>
   __device__ __forceinline__ void operator()(float (&x)[N]) {
-    if constexpr (kWaves == 1) {
+    if constexpr (!TEAM) {
 #pragma unroll
       for (int n = 0; n < N; ++n) x[n] = of_lane(wave_sum(x[n]), kWave - 1);
     } else {
@@ -276,11 +279,14 @@ struct TeamSums {
         for (int n = 0; n < N; ++n) w[wave][n] = x[n];
       }
       __syncthreads();
-      const int from = lane % 16;
+      const int from = lane % kMostWaves;
 #pragma unroll
-      for (int n = 0; n < N; ++n) x[n] = from < kWaves ? w[from < kWaves ? from : 0][n] : 0.0f;
+      for (int n = 0; n < N; ++n) {
+        x[n] = w[from][n];
+        x[n] = from < waves ? x[n] : 0.0f;  // (words of wavefronts that there are not hold anything)
+      }
 #pragma unroll
-      for (int n = 0; n < N; ++n) x[n] = of_lane(row_sum(x[n]), 15);
+      for (int n = 0; n < N; ++n) x[n] = of_lane(row_sum(x[n]), kMostWaves - 1);
       turn ^= 1;
     }
   }

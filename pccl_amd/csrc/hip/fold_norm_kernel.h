@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "fold_norm_device.h"
+#include "reduce_copy_kernel.h"
 
 namespace pccl_dev {
 
@@ -21,6 +22,8 @@ struct NormArgs {  // both directions
   long in_bytes;
 };
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 struct ForwardArgs : NormArgs {
   unsigned row0;  // the launch's first row
   const char *residual;
@@ -29,8 +32,8 @@ struct ForwardArgs : NormArgs {
 };
 
 // v's norm over the team in place: v - mean (layer) and one over the spread; masked elements stay 0.
-template <class R, int LANES, int E>
-__device__ __forceinline__ float standardise(const Share<R, LANES, E> &s, TeamSums<LANES> &sums, int kind, float per_width, float eps,
+template <class R, bool TEAM, int E>
+__device__ __forceinline__ float standardise(const Share<R, TEAM, E> &s, TeamSums<TEAM> &sums, int kind, float per_width, float eps,
                                              float (&v)[E]) {
   float t[1];
   if (kind == PCCL_NORM_LAYER) {  // two passes over the registers: no cancellation between E[v^2] and E[v]^2
@@ -51,8 +54,8 @@ __device__ __forceinline__ float standardise(const Share<R, LANES, E> &s, TeamSu
 }
 
 // x = v * rstd * (weight + offset) + bias
-template <class R, bool PF32, int LANES, int E>
-__device__ __forceinline__ void scale_and_shift(const Share<R, LANES, E> &s, const ParamShare<R, PF32, LANES, E> &weight, bool has_weight,
+template <class R, bool PF32, bool TEAM, int E>
+__device__ __forceinline__ void scale_and_shift(const Share<R, TEAM, E> &s, const ParamShare<R, PF32, TEAM, E> &weight, bool has_weight,
                                                 float offset, const char *bias, float rstd, float (&v)[E]) {
 #pragma unroll
   for (int i = 0; i < E; ++i) v[i] *= rstd;
@@ -63,7 +66,7 @@ __device__ __forceinline__ void scale_and_shift(const Share<R, LANES, E> &s, con
     for (int i = 0; i < E; ++i) v[i] *= w[i] + offset;
   }
   if (bias) {
-    ParamShare<R, PF32, LANES, E> b;
+    ParamShare<R, PF32, TEAM, E> b;
     float x[E];
     b.load(s, bias);
     b.up(x);
@@ -72,25 +75,27 @@ __device__ __forceinline__ void scale_and_shift(const Share<R, LANES, E> &s, con
   }
 }
 
-// Lanes of a workgroup: teams of one wavefront come four to a workgroup (they meet at no barrier), others have their own.
-constexpr int team_block(int lanes) { return lanes == kWave ? kBlock : lanes; }
+constexpr int kMostLanes = kMostWaves * kWave;
+constexpr int team_block(bool team) { return team ? kMostLanes : kBlock; }  // lanes of a workgroup, at most
 
-template <int DT, bool PF32, int LANES, int E, int AT_ONCE>
-__global__ void __launch_bounds__(team_block(LANES)) fold_norm_kernel(const ForwardArgs a) {
+// STREAM: the inputs are read non-temporally.  Workgroups of the launch take rows in the order of rotated_chunk, for the reasons given
+// there (8 -> 8 bf16 at 2048 x 8192 119 -> 111 us, 8 -> 1 at 4096 x 4096 64 -> 61, narrow rows unchanged).
+template <int DT, bool PF32, bool TEAM, int E, int AT_ONCE, bool STREAM>
+__global__ void __launch_bounds__(team_block(TEAM)) fold_norm_kernel(const ForwardArgs a) {
   typedef RowType<DT> R;
-  constexpr int kTeams = team_block(LANES) / LANES;
-  __shared__ float words[2][LANES / kWave][kSumsAtOnce];
-  const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / LANES);
-  const unsigned row = a.row0 + blockIdx.x * kTeams + team;
+  constexpr int kTeams = TEAM ? 1 : kBlock / kWave;
+  __shared__ float words[2][TEAM ? kMostWaves : 1][kSumsAtOnce];
+  const int team = TEAM ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lanes = TEAM ? (int)blockDim.x : kWave;
+  const unsigned row = a.row0 + rotated_chunk(blockIdx.x, gridDim.x) * kTeams + team;
   if (row >= a.rows) return;  // a whole team; teams of one wavefront meet at no barrier
-  const Share<R, LANES, E> s((int)threadIdx.x % LANES, a.width);
-  TeamSums<LANES> sums{words, 0};
+  const Share<R, TEAM, E> s((int)threadIdx.x % lanes, lanes, a.width);
+  TeamSums<TEAM> sums{words, lanes / kWave, 0};
 
-  ParamShare<R, PF32, LANES, E> post_weight, pre_weight, gate;
+  ParamShare<R, PF32, TEAM, E> post_weight, pre_weight, gate;
   u32x4 x[E / R::kPack];
   float v[E];
-  if (a.residual) s.load(a.residual + (long)row * a.residual_bytes, x);
-  fold_rows<R, LANES, E, AT_ONCE>(s, a.ins, a.n_in, (long)row * a.in_bytes, v);
+  if (a.residual) s.template load<STREAM>(a.residual + (long)row * a.residual_bytes, x);
+  fold_rows<STREAM, AT_ONCE>(s, a.ins, a.n_in, (long)row * a.in_bytes, v);
   s.mask(v);
   // parameters come from the caches; asked for in front of the sums that they are waited for behind
   if (a.post_weight) post_weight.load(s, a.post_weight);
@@ -130,16 +135,17 @@ __global__ void __launch_bounds__(team_block(LANES)) fold_norm_kernel(const Forw
 }
 
 // ---- backward ----------------------------------------------------------------------------------------
-// The rows are cut into strips that lie within the rows of one gate row (strips of a gate row: `strips`, of
-// `strip_rows` rows; without a gate all rows count as one gate row's), and a team goes through consecutive
-// strips.  Lane l holds the same columns of every row, so the sums over rows stay in its registers; a team
-// writes those of the parameters once, at its end, and those of the gate at the end of each strip.
+// The rows of one gate row (without a gate: all rows) are dealt out to `strips` strips, row i to strip i mod strips, and a
+// team goes through consecutive strips.  Teams at work at the same time so read neighbouring rows: a window that moves through
+// memory in address order.  (With strips of consecutive rows the teams stood a power of two of bytes apart, bf16
+// 16384 x 8192 at 64 rows a team 1 MiB, and fell on the same channels.)  Lane l holds the same columns of every row, so the sums over
+// rows stay in its registers; a team writes those of the parameters once, at its end, and those of the gate at the end of each strip.
 struct BackwardArgs : NormArgs {
   const char *residual_out, *grad_residual_out, *grad_outs[PCCL_MAX_OUTPUTS];
   char *grad_residual, *grad_ins[PCCL_MAX_INPUTS];
   int n_grad_in;
   long residual_out_bytes, grad_residual_out_bytes, grad_out_bytes, grad_residual_bytes, grad_in_bytes;
-  unsigned n_strips, strip_rows;  // in all; rows of one
+  unsigned n_strips;              // in all
   unsigned strips;                // of one gate row
   unsigned n_teams;
   // what the sums over rows go to: [n_teams][4][width] (post weight, post bias, pre weight, pre bias) and, with
@@ -150,8 +156,9 @@ struct BackwardArgs : NormArgs {
   bool want_sums[4];
 };
 
-template <class R, int LANES, int E>
-__device__ __forceinline__ void store_sums(const Share<R, LANES, E> &s, float *row, const float (&x)[E]) {
+// A lane's share of a row of sums in the workspace (binary32).
+template <class R, bool TEAM, int E>
+__device__ __forceinline__ void store_sums(const Share<R, TEAM, E> &s, float *row, const float (&x)[E]) {
 #pragma unroll
   for (int j = 0; j < E / R::kPack; ++j) {
     if (s.lo[j] == 0) {
@@ -166,14 +173,43 @@ __device__ __forceinline__ void store_sums(const Share<R, LANES, E> &s, float *r
   }
 }
 
-// x = the lane's share of a row of sums, or zeros
-template <class R, int LANES, int E>
-__device__ __forceinline__ void load_sums(const Share<R, LANES, E> &s, const float *row, bool there, float (&x)[E]) {
+// Sums over rows that a lane keeps for its columns, in registers or (IN_LDS) in the workgroup's LDS, four columns to a 16-byte
+// word, words of one lane `step` apart.
+template <int E, bool IN_LDS>
+struct Columns {
+  float x[IN_LDS ? 1 : E];
+  f32x4 *at;
+  int step;
+
+  __device__ __forceinline__ void zero() {
+    if constexpr (IN_LDS) {
 #pragma unroll
-  for (int j = 0; j < E / R::kPack; ++j)
+      for (int k = 0; k < E / 4; ++k) at[k * step] = f32x4{0, 0, 0, 0};
+    } else {
 #pragma unroll
-    for (int i = 0; i < R::kPack; ++i) x[j * R::kPack + i] = there && i >= s.lo[j] ? row[s.off[j] + i] : 0.0f;
-}
+      for (int i = 0; i < E; ++i) x[i] = 0.0f;
+    }
+  }
+  // += a * b, element by element
+  __device__ __forceinline__ void add(const float (&a)[E], const float (&b)[E]) {
+    if constexpr (IN_LDS) {
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k) {
+        f32x4 v = at[k * step];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(a[4 * k + i], b[4 * k + i], v[i]);
+        at[k * step] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(a[i], b[i], x[i]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&to)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) to[i] = IN_LDS ? at[i / 4 * step][i % 4] : x[i];
+  }
+};
 
 // What a row of the backward pass sums over the team: a parameter's column sums come from two products per element.
 // With yhat, rhat the standardised y and r:
@@ -183,9 +219,13 @@ __device__ __forceinline__ void load_sums(const Share<R, LANES, E> &s, const flo
 //   p1 = sum dh * rhat, p0 = sum dh  weight and bias of the pre norm
 // so that a row costs one fused multiply-add a column for each, and gate and weight are met once a strip.
 //
-// One team's registers hold the row (packed), the row after it on its way (SINGLE: one y and at most one dh, so that
-// four streams are read), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, and the sums.
+// One team's registers hold the row (packed), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, s1 and p1.
+// 16-bit rows of up to 8192 columns (E = 8) that are four streams (SINGLE: one y and at most one dh) have room for the row
+// after it, on its way; binary32 rows spilled with it (8192 x 2048 87 -> 84 us without).  s0 and p0 and the post norm's sums over a
+// team's strips stay in LDS.  Wider rows (E = 16) keep s1 and p1 there instead, the post norm's sums over strips go to the
+// workspace and back.
 // BIAS: some bias's gradient or a gate behind a biased norm is asked for (s0 and p0 are kept).
+// STREAM: rows are read non-temporally.
 //
 // The arguments (18 addresses and 12 strides) are read again from the argument segment wherever a row needs them: held
 // in scalar registers over the loop they spill into vector registers, and those are what is short here.
@@ -194,106 +234,120 @@ __device__ __forceinline__ BackwardArgsAt read_again(BackwardArgsAt p) {
   asm volatile("" : "+s"(p));  // (no instruction: the compiler may not know what it points to any more)
   return p;
 }
-template <class R, int LANES, int E>
+template <class R, int E>
 struct BackRow {
   u32x4 y[E / R::kPack], r[E / R::kPack], dh[E / R::kPack], dr[E / R::kPack];
 };
 
-template <int DT, bool PF32, int LANES, int E, bool SINGLE, bool BIAS>
-__global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kernel(const BackwardArgs) {
+template <int DT, int E>
+constexpr bool row_ahead() { return DT != PCCL_F32 && E == 8; }
+
+template <int DT, bool PF32, bool TEAM, int E, bool SINGLE, bool BIAS, bool STREAM>
+__global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel(const BackwardArgs) {
   typedef RowType<DT> R;
-  typedef Share<R, LANES, E> S;
-  typedef ParamShare<R, PF32, LANES, E> P;
-  constexpr int kTeams = team_block(LANES) / LANES;
+  typedef Share<R, TEAM, E> S;
+  typedef ParamShare<R, PF32, TEAM, E> P;
+  constexpr int kTeams = TEAM ? 1 : kBlock / kWave;
+  constexpr bool kWide = E > 8;
   constexpr int kFold = 4;  // gradients in flight together; more cost registers
   const BackwardArgsAt args = (BackwardArgsAt)__builtin_amdgcn_kernarg_segment_ptr();  // (the one argument stands at its start)
   const BackwardArgsAt a0 = args;
-  __shared__ float words[2][LANES / kWave][kSumsAtOnce];
-  const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / LANES);
+  __shared__ float words[2][TEAM ? kMostWaves : 1][kSumsAtOnce];
+  extern __shared__ f32x4 column_words[];  // backward_lds() of them
+  const int team = TEAM ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lanes = TEAM ? (int)blockDim.x : kWave;
   const unsigned t = blockIdx.x * kTeams + team;
-  if (t >= a0->n_teams) return;
-  const S s((int)threadIdx.x % LANES, a0->width);
-  TeamSums<LANES> sums{words, 0};
+  const bool there = t < a0->n_teams;  // (a workgroup's last teams may have nothing to do, but they meet the others at its end)
+  const S s((int)threadIdx.x % lanes, lanes, a0->width);
+  TeamSums<TEAM> sums{words, lanes / kWave, 0};
+  auto columns = [&](int n) { return column_words + (n * (E / 4)) * (int)blockDim.x + (int)threadIdx.x; };
   const bool post = a0->post_kind != PCCL_NORM_NONE, outs = a0->n_out > 0, pre = a0->pre_kind != PCCL_NORM_NONE && outs;
   const bool post_layer = a0->post_kind == PCCL_NORM_LAYER, pre_layer = pre && a0->pre_kind == PCCL_NORM_LAYER;
   const float per_width = a0->per_width;
 
-  float wpre[E], p1[E], p0[BIAS ? E : 1];
+  float wpre_kept[kWide ? 1 : E], ones[E];
+  Columns<E, kWide> p1{{}, columns(0), (int)blockDim.x}, s1{{}, columns(1), (int)blockDim.x};
+  Columns<E, !kWide> p0{{}, columns(2), (int)blockDim.x}, s0{{}, columns(3), (int)blockDim.x};                   // (BIAS)
+  Columns<E, true> post_sums{{}, columns(0), (int)blockDim.x}, post_bias_sums{{}, columns(1), (int)blockDim.x};  // (E = 8)
+  p1.zero();
+  if constexpr (BIAS) p0.zero();
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    wpre[i] = 1.0f;
-    p1[i] = 0.0f;
-    if constexpr (BIAS) p0[i] = 0.0f;
-  }
-  if (a0->pre_weight) {
-    P w;
-    w.load(s, a0->pre_weight);
-    w.up(wpre);
-#pragma unroll
-    for (int i = 0; i < E; ++i) wpre[i] += a0->weight_offset;
-  }
-
-  auto load_row = [&](unsigned long row, BackRow<R, LANES, E> &x) {
+  for (int i = 0; i < E; ++i) ones[i] = 1.0f;
+  // wpre and cgw: with E = 16 read again (from the caches) wherever a row needs them
+  auto get_wpre = [&](float (&to)[E]) {
     const BackwardArgsAt a = read_again(args);
-    if (a->grad_residual_out) s.load(a->grad_residual_out + row * a->grad_residual_out_bytes, x.dr);
-    if (pre) s.load(a->residual_out + row * a->residual_out_bytes, x.r);
+#pragma unroll
+    for (int i = 0; i < E; ++i) to[i] = 1.0f;
+    if (a->pre_weight) {
+      P w;
+      w.load(s, a->pre_weight);
+      w.up(to);
+#pragma unroll
+      for (int i = 0; i < E; ++i) to[i] += a->weight_offset;
+    }
+  };
+  auto get_cgw = [&](unsigned group, float (&to)[E]) {
+    const BackwardArgsAt a = read_again(args);
+#pragma unroll
+    for (int i = 0; i < E; ++i) to[i] = a->block_scale;
+    if (a->gate) {
+      P g;
+      float f[E];
+      g.load(s, a->gate + group * a->gate_bytes);
+      g.up(f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) to[i] *= f[i];
+    }
+    if (a->post_weight) {
+      P w;
+      float f[E];
+      w.load(s, a->post_weight);
+      w.up(f);
+#pragma unroll
+      for (int i = 0; i < E; ++i) to[i] *= f[i] + a->weight_offset;
+    }
+  };
+  if constexpr (!kWide) get_wpre(wpre_kept);
+
+  auto load_row = [&](unsigned long row, BackRow<R, E> &x) {
+    const BackwardArgsAt a = read_again(args);
+    if (a->grad_residual_out) s.template load<STREAM>(a->grad_residual_out + row * a->grad_residual_out_bytes, x.dr);
+    if (pre) s.template load<STREAM>(a->residual_out + row * a->residual_out_bytes, x.r);
     if constexpr (SINGLE) {
-      if (outs) s.load(a->grad_outs[0] + row * a->grad_out_bytes, x.dh);
-      s.load(a->ins[0] + row * a->in_bytes, x.y);
+      if (outs) s.template load<STREAM>(a->grad_outs[0] + row * a->grad_out_bytes, x.dh);
+      s.template load<STREAM>(a->ins[0] + row * a->in_bytes, x.y);
     }
   };
 
   const unsigned first = (unsigned)((unsigned long)a0->n_strips * t / a0->n_teams);
-  const unsigned end = (unsigned)((unsigned long)a0->n_strips * (t + 1) / a0->n_teams);
+  const unsigned end = there ? (unsigned)((unsigned long)a0->n_strips * (t + 1) / a0->n_teams) : first;
   for (unsigned strip = first; strip < end; ++strip) {
     const BackwardArgsAt a1 = read_again(args);
     const unsigned group = strip / a1->strips;
-    // (the last gate row may have fewer rows than gate_rows, and its last strips then none: 64 bits, and no row)
-    const unsigned long group_row = (unsigned long)group * a1->gate_rows;
-    const unsigned long begin = group_row + (unsigned long)(strip - group * a1->strips) * a1->strip_rows;
-    unsigned long stop = begin + a1->strip_rows;
-    if (stop > group_row + a1->gate_rows) stop = group_row + a1->gate_rows;
+    const unsigned long group_row = (unsigned long)group * a1->gate_rows, begin = group_row + (strip - group * a1->strips);
+    unsigned long stop = group_row + a1->gate_rows;  // (the last gate row may have fewer rows than gate_rows, and some of its strips none)
     if (stop > a1->rows) stop = a1->rows;
+    const unsigned step = a1->strips;
 
-    BackRow<R, LANES, E> next;
+    BackRow<R, E> next;
     if (SINGLE && begin < stop) load_row(begin, next);
-    float cgw[E], s1[E], s0[BIAS ? E : 1];
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      cgw[i] = a1->block_scale;
-      s1[i] = 0.0f;
-      if constexpr (BIAS) s0[i] = 0.0f;
-    }
-    if (a1->gate) {
-      P g;
-      float f[E];
-      g.load(s, a1->gate + group * a1->gate_bytes);
-      g.up(f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) cgw[i] *= f[i];
-    }
-    if (a1->post_weight) {
-      P w;
-      float f[E];
-      w.load(s, a1->post_weight);
-      w.up(f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) cgw[i] *= f[i] + a1->weight_offset;
-    }
+    s1.zero();
+    if constexpr (BIAS) s0.zero();
+    float cgw_kept[kWide ? 1 : E];
+    if constexpr (!kWide) get_cgw(group, cgw_kept);
 
-    for (unsigned long row = begin; row < stop; ++row) {
-      BackRow<R, LANES, E> now;
+    for (unsigned long row = begin; row < stop; row += step) {
+      BackRow<R, E> now;
       float y[E], dh[E], r[E];
       if constexpr (SINGLE) {
         now = next;
-        if (row + 1 < stop) load_row(row + 1, next);
+        if (row + step < stop) load_row(row + step, next);
         s.up(now.y, y);
         if (outs) s.up(now.dh, dh);
       } else {
         load_row(row, now);
         const BackwardArgsAt a = read_again(args);
-        if (outs) fold_rows<R, LANES, E, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh);
-        fold_rows<R, LANES, E, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y);
+        if (outs) fold_rows<STREAM, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh);
+        fold_rows<STREAM, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y);
       }
       s.mask(y);
       if (outs) s.mask(dh);
@@ -332,6 +386,9 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
         for (int i = 0; i < E; ++i) q[0] = __builtin_fmaf(y[i], y[i], q[0]);
       }
       if (pre) {
+        float w[kWide ? E : 1];
+        if constexpr (kWide) get_wpre(w);
+        const auto &wpre = [&]() -> const float (&)[E] { if constexpr (kWide) return w; else return wpre_kept; }();
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           q[1] = __builtin_fmaf(r[i], r[i], q[1]);
@@ -355,20 +412,21 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
         // dr += rstd * (d - rhat * mean(d * rhat) - mean(d)), d = dh * w
         const float rstd = one_over_spread(q[1], per_width, a->pre_eps);
         const float along = -(rstd * rstd * rstd) * (q[2] * per_width);
+        float w[kWide ? E : 1];
+        if constexpr (kWide) get_wpre(w);
+        const auto &wpre = [&]() -> const float (&)[E] { if constexpr (kWide) return w; else return wpre_kept; }();
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          p1[i] = __builtin_fmaf(dh[i], r[i] * rstd, p1[i]);
           dr[i] = __builtin_fmaf(dh[i] * wpre[i], rstd, __builtin_fmaf(r[i], along, dr[i]));
+          r[i] *= rstd;
         }
+        p1.add(dh, r);
         if (pre_layer) {
           const float mean = rstd * (q[3] * per_width);
 #pragma unroll
           for (int i = 0; i < E; ++i) dr[i] -= mean;
         }
-        if constexpr (BIAS) {
-#pragma unroll
-          for (int i = 0; i < E; ++i) p0[i] += dh[i];
-        }
+        if constexpr (BIAS) p0.add(dh, ones);
       } else if (outs) {
 #pragma unroll
         for (int i = 0; i < E; ++i) dr[i] += dh[i];
@@ -380,18 +438,16 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
         for (int i = 0; i < E; ++i) x[i] = a->residual_scale * dr[i];
         s.store(a->grad_residual + row * a->grad_residual_bytes, x);
       }
+      float cgw_read[kWide ? E : 1];
+      if constexpr (kWide) get_cgw(group, cgw_read);
+      const auto &cgw = [&]() -> const float (&)[E] { if constexpr (kWide) return cgw_read; else return cgw_kept; }();
       if (post) {
         const float rstd = one_over_spread(q[0], per_width, a->post_eps);
         float m[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          y[i] *= rstd;
-          s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
-        }
-        if constexpr (BIAS) {
-#pragma unroll
-          for (int i = 0; i < E; ++i) s0[i] += dr[i];
-        }
+        for (int i = 0; i < E; ++i) y[i] *= rstd;
+        s1.add(dr, y);
+        if constexpr (BIAS) s0.add(dr, ones);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           dr[i] *= cgw[i];
@@ -406,11 +462,9 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
 #pragma unroll
         for (int i = 0; i < E; ++i) dr[i] = __builtin_fmaf(dr[i], rstd, __builtin_fmaf(y[i], along, mean));
       } else {
+        s1.add(dr, y);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
-          dr[i] *= cgw[i];
-        }
+        for (int i = 0; i < E; ++i) dr[i] *= cgw[i];
       }
       const unsigned long at = row * a->grad_in_bytes;
 #pragma unroll 1
@@ -419,17 +473,20 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
 
     // the strip's sums: to the gate's gradient or its workspace, and, times the gate, to the team's
     const BackwardArgsAt a = read_again(args);
+    float x[E], x0[E];
+    s1.get(x);
+    if constexpr (BIAS) s0.get(x0);
     if (a->grad_gate) {
-      float x[E];
+      float d[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = s1[i] * a->block_scale;
+      for (int i = 0; i < E; ++i) d[i] = x[i] * a->block_scale;
       if (a->post_weight) {
         P w;
         float f[E];
         w.load(s, a->post_weight);
         w.up(f);
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] *= f[i] + a->weight_offset;
+        for (int i = 0; i < E; ++i) d[i] *= f[i] + a->weight_offset;
       }
       if constexpr (BIAS) {
         if (a->post_bias) {
@@ -438,15 +495,15 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
           b.load(s, a->post_bias);
           b.up(f);
 #pragma unroll
-          for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i] * a->block_scale, s0[i], x[i]);
+          for (int i = 0; i < E; ++i) d[i] = __builtin_fmaf(f[i] * a->block_scale, x0[i], d[i]);
         }
       }
       if (a->gate_sums) {
-        store_sums(s, a->gate_sums + (unsigned long)strip * a->width, x);
+        store_sums(s, a->gate_sums + (unsigned long)strip * a->width, d);
       } else if constexpr (PF32 && R::kBytes == 2) {
-        store_sums(s, (float *)(a->grad_gate + group * a->grad_gate_bytes), x);
+        store_sums(s, (float *)(a->grad_gate + group * a->grad_gate_bytes), d);
       } else {
-        s.store(a->grad_gate + group * a->grad_gate_bytes, x);
+        s.store(a->grad_gate + group * a->grad_gate_bytes, d);
       }
     }
     if (a->want_sums[0] || a->want_sums[1]) {
@@ -455,131 +512,198 @@ __global__ void __launch_bounds__(team_block(LANES), 4) fold_norm_backward_kerne
       for (int i = 0; i < E; ++i) f[i] = a->block_scale;
       if (a->gate) {
         P g;
-        float x[E];
+        float e[E];
         g.load(s, a->gate + group * a->gate_bytes);
-        g.up(x);
+        g.up(e);
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] *= x[i];
+        for (int i = 0; i < E; ++i) f[i] *= e[i];
       }
-      // a team of several strips adds to what it wrote itself (each lane to its own columns)
-      float *mine = a->sums + (unsigned long)t * 4 * a->width;
-      float x[E];
-      if (a->want_sums[0]) {
-        load_sums(s, mine, strip != first, x);
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i], s1[i], x[i]);
-        store_sums(s, mine, x);
-      }
-      if constexpr (BIAS) {
-        if (a->want_sums[1]) {
-          load_sums(s, mine + a->width, strip != first, x);
-#pragma unroll
-          for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(f[i], s0[i], x[i]);
-          store_sums(s, mine + a->width, x);
+      if constexpr (!kWide) {
+        if (strip == first) {
+          post_sums.zero();
+          if constexpr (BIAS) post_bias_sums.zero();
         }
+        post_sums.add(f, x);
+        if constexpr (BIAS) post_bias_sums.add(f, x0);
+      } else {
+        // (each lane adds to the columns that it wrote itself)
+        float *mine = a->sums + (unsigned long)t * 4 * a->width;
+        auto add = [&](float *row, const float (&v)[E]) {
+          float had[E];
+#pragma unroll
+          for (int j = 0; j < E / R::kPack; ++j)
+#pragma unroll
+            for (int i = 0; i < R::kPack; ++i)
+              had[j * R::kPack + i] = strip != first && i >= s.lo[j] ? row[s.off[j] + i] : 0.0f;
+#pragma unroll
+          for (int i = 0; i < E; ++i) had[i] = __builtin_fmaf(f[i], v[i], had[i]);
+          store_sums(s, row, had);
+        };
+        if (a->want_sums[0]) add(mine, x);
+        if constexpr (BIAS)
+          if (a->want_sums[1]) add(mine + a->width, x0);
       }
     }
   }
-  float *mine = a0->sums + (unsigned long)t * 4 * a0->width;
-  if (a0->want_sums[2]) store_sums(s, mine + 2 * a0->width, p1);
-  if constexpr (BIAS) {
-    if (a0->want_sums[3]) store_sums(s, mine + 3 * a0->width, p0);
+  // the team's sums; those of the four teams of a workgroup are added first
+  float *mine = a0->sums + (unsigned long)(TEAM ? t : blockIdx.x) * 4 * a0->width;
+  auto put = [&](int which, bool set, float (&x)[E]) {
+    if constexpr (!TEAM) {
+      __syncthreads();  // (every team comes here; what LDS held before is done with)
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k) column_words[k * kBlock + (int)threadIdx.x] = set ? f32x4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]} : f32x4{0, 0, 0, 0};
+      __syncthreads();
+      if (team != 0) return;
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = column_words[i / 4 * kBlock + (int)threadIdx.x][i % 4];
+#pragma unroll
+      for (int other = 1; other < kTeams; ++other)
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] += column_words[i / 4 * kBlock + other * kWave + (int)threadIdx.x][i % 4];
+    }
+    store_sums(s, mine + which * a0->width, x);
+  };
+  // (taken out of LDS before the first of them goes through it)
+  float x_post[E], x_post_bias[E], x_p1[E], x_p0[E];
+  if constexpr (!kWide) post_sums.get(x_post);
+  if constexpr (!kWide && BIAS) post_bias_sums.get(x_post_bias);
+  p1.get(x_p1);
+  if constexpr (BIAS) p0.get(x_p0);
+  if constexpr (!kWide) {  // (a team has a strip, so these were set)
+    if (a0->want_sums[0]) put(0, there, x_post);
+    if constexpr (BIAS)
+      if (a0->want_sums[1]) put(1, there, x_post_bias);
   }
+  if (a0->want_sums[2]) put(2, there, x_p1);
+  if constexpr (BIAS)
+    if (a0->want_sums[3]) put(3, there, x_p0);
 }
 
-// Joins the teams' sums: a workgroup adds 64 columns of one parameter's (or one gate row's) partial rows, 16 wavefronts
-// every sixteenth row each, then the 16 in order.
+// Bytes of LDS for sums by column: with E = 8 the post norm's, with biases theirs, p0 and s0 too; with E = 16 p1 and s1.
+inline unsigned backward_lds(int lanes_of_workgroup, int elems, bool bias) {
+  return (unsigned)lanes_of_workgroup * elems * 4 * (elems > 8 ? 2 : bias ? 4 : 1);
+}
+
+// Joins the teams' sums: a workgroup adds 64 columns of one parameter's (or one gate row's) partial rows.  A lane has four columns, so
+// that four rows of 256 bytes are one load of a wavefront and sixteen wavefronts have 64 rows at work at once, each every 64th
+// row; then the four of a wavefront, then the wavefronts, always in the same order.  What bounds it is the round trip to memory (the
+// rows were written by other chiplets): few workgroups, all resident, eight loads of each lane in flight.  (One column a lane and 16 or 64
+// columns a workgroup: 512 rows x 4096 x 8 20 us, 1024 rows x 300 x 2 9 us and, with 64, 17.)
 struct SumsArgs {
   const float *sums, *gate_sums;
   char *out[4];      // by parameter, null: not wanted
   int listed[4];     // which parameters blockIdx.y = 0 .. n_listed - 1 stand for
   int n_listed, width;
-  unsigned n_teams, strips;
+  unsigned n_partial, strips;
   char *grad_gate;   // blockIdx.y = n_listed + gate row
   long grad_gate_bytes;
 };
-constexpr int kJoinWaves = 16;
+constexpr int kJoinWaves = 16, kJoinColumns = 64, kJoinRows = 4;
 
 template <int DT, bool PF32>
 __global__ void __launch_bounds__(kJoinWaves * kWave) fold_norm_sums_kernel(const SumsArgs a) {
-  __shared__ float part[kJoinWaves][kWave];
-  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
-  const int column = (int)blockIdx.x * kWave + lane;
+  __shared__ f32x4 part[kJoinWaves][kWave / kJoinRows];
+  const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave, at = lane % (kWave / kJoinRows);
+  // the last lanes move back to end with the row: they add, and store, what their neighbours do (rows of less than four: one by one)
+  int column = (int)blockIdx.x * kJoinColumns + at * 4;
+  const bool mine = column < a.width, narrow = a.width < 4;
+  if (!narrow && column > a.width - 4) column = a.width - 4;
   const bool of_gate = (int)blockIdx.y >= a.n_listed;
   const int which = of_gate ? 0 : a.listed[blockIdx.y];
   const long group = (int)blockIdx.y - a.n_listed;
   const float *from = of_gate ? a.gate_sums + group * a.strips * a.width : a.sums + (long)which * a.width;
   const long step = of_gate ? a.width : 4l * a.width;
-  const unsigned n = of_gate ? a.strips : a.n_teams;
-  float t = 0.0f;
-  if (column < a.width) {
+  const unsigned n = of_gate ? a.strips : a.n_partial;
+  f32x4 t{0, 0, 0, 0};
+  if (mine) {
+    if (!narrow) {
+      typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 #pragma unroll 8
-    for (unsigned k = wave; k < n; k += kJoinWaves) t += from[k * step + column];
+      for (unsigned k = wave * kJoinRows + lane / (kWave / kJoinRows); k < n; k += kJoinWaves * kJoinRows) t += *(const f32x4_a4 *)(from + k * step + column);
+    } else {
+      for (unsigned k = wave * kJoinRows + lane / (kWave / kJoinRows); k < n; k += kJoinWaves * kJoinRows)
+        for (int i = 0; i < a.width; ++i) t[i] += from[k * step + i];
+    }
   }
-  part[wave][lane] = t;
-  __syncthreads();
-  if (wave != 0 || column >= a.width) return;
 #pragma unroll
-  for (int k = 1; k < kJoinWaves; ++k) t += part[k][lane];
+  for (int i = 0; i < 4; ++i) {
+    t[i] += __shfl_xor(t[i], 16, kWave);
+    t[i] += __shfl_xor(t[i], 32, kWave);
+  }
+  if (lane == at) part[wave][at] = t;
+  __syncthreads();
+  if (wave != 0 || lane != at || !mine) return;
+  t = part[0][at];
+#pragma unroll
+  for (int k = 1; k < kJoinWaves; ++k) t += part[k][at];
   char *to = of_gate ? a.grad_gate + group * a.grad_gate_bytes : a.out[which];
-  if constexpr (PF32) ((float *)to)[column] = t;
-  else ((typename RowType<DT>::elem_t *)to)[column] = RowType<DT>::down1(t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (column + i >= a.width) break;
+    if constexpr (PF32) ((float *)to)[column + i] = t[i];
+    else ((typename RowType<DT>::elem_t *)to)[column + i] = RowType<DT>::down1(t[i]);
+  }
 }
 
 // ---- launchers, one translation unit per pair of types ---------------------------------------------------
-// Lanes of a team and elements a lane, by width.
+// The lanes of a row's team and the elements of a lane.
 struct NormShape {
   int lanes, elems;
+  int block() const { return lanes == kWave ? kBlock : lanes; }  // lanes of a workgroup
+  unsigned workgroups(unsigned rows) const { return lanes == kWave ? (rows + kBlock / kWave - 1) / (kBlock / kWave) : rows; }
 };
 
 template <class F>
-inline bool with_norm_shape(NormShape n, F &&f) {
-#define PCCL_NORM_SHAPE(L, E)                                                              \
-  if (n.lanes == L && n.elems == E) {                                                      \
-    f(std::integral_constant<int, L>{}, std::integral_constant<int, E>{});                 \
-    return true;                                                                           \
-  }
-  PCCL_NORM_SHAPE(64, 8)
-  PCCL_NORM_SHAPE(128, 8)
-  PCCL_NORM_SHAPE(256, 8)
-  PCCL_NORM_SHAPE(512, 8)
-  PCCL_NORM_SHAPE(1024, 8)
-  PCCL_NORM_SHAPE(1024, 16)
-#undef PCCL_NORM_SHAPE
-  return false;
+inline void with_norm_shape(NormShape n, F &&f) {
+  typedef std::integral_constant<int, 8> Eight;
+  typedef std::integral_constant<int, 16> Sixteen;
+  if (n.lanes == kWave) f(std::false_type{}, Eight{});
+  else if (n.elems == 8) f(std::true_type{}, Eight{});
+  else f(std::true_type{}, Sixteen{});
 }
 
-template <int DT, bool PF32> hipError_t launch_fold_norm(NormShape n, hipStream_t stream, const ForwardArgs &a);
-template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool bias, hipStream_t stream, const BackwardArgs &a);
+template <int DT, bool PF32> hipError_t launch_fold_norm(NormShape n, bool stream_in, hipStream_t stream, const ForwardArgs &a);
+template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a);
 template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, hipStream_t stream, const SumsArgs &a);
 
-#define PCCL_DEFINE_FOLD_NORM(DT, PF32)                                                                                     \
-  template <> hipError_t launch_fold_norm<DT, PF32>(NormShape n, hipStream_t stream, const ForwardArgs &a) {                \
-    with_norm_shape(n, [&](auto l, auto e) {                                                                                \
-      constexpr int L = decltype(l)::value, E = decltype(e)::value, kTeams = team_block(L) / L;                             \
-      const unsigned grid = (a.rows - a.row0 + kTeams - 1) / kTeams;                                                        \
-      if (a.n_in <= 2) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, L, E, 2>), dim3(grid), dim3(team_block(L)), 0, stream, a); \
-      else hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, L, E, 8>), dim3(grid), dim3(team_block(L)), 0, stream, a);        \
-    });                                                                                                                     \
-    return hipGetLastError();                                                                                               \
-  }                                                                                                                         \
-  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool bias, hipStream_t stream, const BackwardArgs &a) { \
-    with_norm_shape(n, [&](auto l, auto e) {                                                                                \
-      constexpr int L = decltype(l)::value, E = decltype(e)::value, kTeams = team_block(L) / L;                             \
-      const unsigned grid = (a.n_teams + kTeams - 1) / kTeams;                                                              \
-      const bool single = a.n_in == 1 && a.n_out <= 1;                                                                      \
-      auto run = [&](auto sg, auto b) {                                                                                     \
-        hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, L, E, decltype(sg)::value, decltype(b)::value>), dim3(grid), \
-                           dim3(team_block(L)), 0, stream, a);                                                              \
-      };                                                                                                                    \
-      if (single) bias ? run(std::true_type{}, std::true_type{}) : run(std::true_type{}, std::false_type{});                \
-      else bias ? run(std::false_type{}, std::true_type{}) : run(std::false_type{}, std::false_type{});                     \
-    });                                                                                                                     \
-    return hipGetLastError();                                                                                               \
-  }                                                                                                                         \
-  template <> hipError_t launch_fold_norm_sums<DT, PF32>(unsigned grid_y, hipStream_t stream, const SumsArgs &a) {          \
-    hipLaunchKernelGGL((fold_norm_sums_kernel<DT, PF32>), dim3((a.width + kWave - 1) / kWave, grid_y), dim3(kJoinWaves * kWave), 0, stream, a); \
-    return hipGetLastError();                                                                                               \
+#define PCCL_DEFINE_FOLD_NORM(DT, PF32)                                                                                         \
+  template <> hipError_t launch_fold_norm<DT, PF32>(NormShape n, bool stream_in, hipStream_t stream, const ForwardArgs &a) {    \
+    with_norm_shape(n, [&](auto team, auto e) {                                                                                 \
+      constexpr bool TEAM = decltype(team)::value;                                                                              \
+      constexpr int E = decltype(e)::value;                                                                                     \
+      const dim3 grid(n.workgroups(a.rows - a.row0)), block(n.block());                                                         \
+      if (a.n_in <= 2) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, 2, false>), grid, block, 0, stream, a);          \
+      else if (stream_in) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, 8, true>), grid, block, 0, stream, a);        \
+      else hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, 8, false>), grid, block, 0, stream, a);                      \
+    });                                                                                                                         \
+    return hipGetLastError();                                                                                                   \
+  }                                                                                                                             \
+  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a) { \
+    with_norm_shape(n, [&](auto team, auto e) {                                                                                 \
+      constexpr bool TEAM = decltype(team)::value;                                                                              \
+      constexpr int E = decltype(e)::value;                                                                                     \
+      const dim3 grid(n.workgroups(a.n_teams)), block(n.block());                                                               \
+      const unsigned lds = backward_lds(n.block(), E, bias);                                                                    \
+      auto run = [&](auto single, auto b, auto st) {                                                                            \
+        hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, TEAM, E, decltype(single)::value, decltype(b)::value, decltype(st)::value>), \
+                           grid, block, lds, stream, a);                                                                        \
+      };                                                                                                                        \
+      constexpr bool kAhead = row_ahead<DT, E>();                                                                               \
+      if (kAhead && a.n_in == 1 && a.n_out <= 1) {                                                                              \
+        typedef std::integral_constant<bool, kAhead> Single;                                                                    \
+        if (stream_in) bias ? run(Single{}, std::true_type{}, std::true_type{}) : run(Single{}, std::false_type{}, std::true_type{}); \
+        else bias ? run(Single{}, std::true_type{}, std::false_type{}) : run(Single{}, std::false_type{}, std::false_type{});   \
+      } else {                                                                                                                  \
+        typedef std::integral_constant<bool, !kAhead> Streams; /* (16-bit rows of several gradients: 85 against 88 us, not worth a variant) */ \
+        if (stream_in) bias ? run(std::false_type{}, std::true_type{}, Streams{}) : run(std::false_type{}, std::false_type{}, Streams{}); \
+        else bias ? run(std::false_type{}, std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{}, std::false_type{}); \
+      }                                                                                                                         \
+    });                                                                                                                         \
+    return hipGetLastError();                                                                                                   \
+  }                                                                                                                             \
+  template <> hipError_t launch_fold_norm_sums<DT, PF32>(unsigned grid_y, hipStream_t stream, const SumsArgs &a) {              \
+    hipLaunchKernelGGL((fold_norm_sums_kernel<DT, PF32>), dim3((a.width + kJoinColumns - 1) / kJoinColumns, grid_y), dim3(kJoinWaves * kWave), 0, stream, a); \
+    return hipGetLastError();                                                                                                   \
   }
 
 }  // namespace pccl_dev
