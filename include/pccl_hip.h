@@ -218,7 +218,8 @@ typedef struct pccl_fold_norm_grads {
   long workspace_bytes;
 } pccl_fold_norm_grads;
 
-/* Two kernel launches on `stream` (one if no gradient of a parameter is asked for). */
+/* Two kernel launches on `stream` (one if no gradient of a parameter is asked for).  Rows may be written in place as in the forward
+ * pass; a parameter's gradient has a buffer of its own. */
 int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const pccl_fold_norm_grads *g, void *stream);
 
 /* Bytes of workspace that a backward pass over this many rows needs on the current device, whichever gradients it asks for

@@ -220,6 +220,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
     c.out(g->grad_ins[k], g->grad_in_stride, "a gradient of the inputs", d->rows, c.es);
   }
   c.out(g->grad_residual, g->grad_residual_stride, "grad_residual", d->rows, c.es);
+  if (g->grad_gate && g->grad_gate == d->gate) return fail(PCCL_ERR_INVALID_ARG, "grad_gate is the gate itself");
   if (g->grad_gate && !d->gate) return fail(PCCL_ERR_INVALID_ARG, "gradient of a gate that there is not");
   if (g->grad_gate) c.out(g->grad_gate, g->grad_gate_stride, "grad_gate", gate_row_count(d->rows, d->gate_rows), c.ps);
   const bool has[4] = {d->post_weight != nullptr, d->post_bias != nullptr, d->pre_weight != nullptr, d->pre_bias != nullptr};

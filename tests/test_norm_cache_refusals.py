@@ -81,6 +81,7 @@ def test_norm_gradients():
     refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, grad_residual=A, grad_residual_stride=1, **good)
     refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, grad_gate=A, **good)           # no gate
     refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, gate=A, gate_rows=1, grad_gate=A, grad_gate_stride=1, **good)
+    refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, gate=A, gate_rows=1, grad_gate=A, **good)   # over the gate itself
     refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, grad_pre_bias=A, **good)       # no bias
     need = n.workspace_bytes(2)
     assert "workspace" in refused(hip.ERR_INVALID_ARG, n.backward, [A], [A], [A], 2, grad_pre_weight=A, **good)
@@ -125,6 +126,11 @@ def test_cache_write():
     refused(hip.ERR_MISALIGNED, c.write, "bf16", [A, A + 1], A, 1)
     refused(hip.ERR_MISALIGNED, c.write, "bf16", [A, A], A + 4, 1)
     refused(hip.ERR_INVALID_ARG, c.write, "bf16", [A, A], A, 1, token_stride=-1)
+    refused(hip.ERR_INVALID_ARG, c.write, "bf16", [A, A], A, 1, head_stride=-1)
+    refused(hip.ERR_INVALID_ARG, c.write, "bf16", [A, A], A, 1, head_stride=(1 << 40) + 1)
+    refused(hip.ERR_UNSUPPORTED, c.write, "bf16", [A, A], A, 1, token_stride=1 << 31)
+    refused(hip.ERR_UNSUPPORTED, cache(code_strides=(1 << 32, 128, 64)).write, "bf16", [A, A], A, 1)
+    refused(hip.ERR_UNSUPPORTED, cache(scale_strides=(1 << 32, 4, 2)).write, "bf16", [A, A], A, 1)
     c.write("bf16", [A, A], A, 0)
     c.write("bf16", [None, None], None, 0)
 
@@ -160,6 +166,8 @@ def test_cache_read():
     refused(hip.ERR_INVALID_ARG, r, most=1 << 31)
     refused(hip.ERR_INVALID_ARG, r, stride=-1)
     refused(hip.ERR_INVALID_ARG, r, out_rows=-1)
+    refused(hip.ERR_INVALID_ARG, r, out_rows=1 << 31)
+    refused(hip.ERR_UNSUPPORTED, r, token_stride=1 << 31)
     assert "overlap" in refused(hip.ERR_INVALID_ARG, r, token_stride=127)
     refused(hip.ERR_INVALID_ARG, r, head_stride=63)
     r(n=0, table=None, lengths=None)
