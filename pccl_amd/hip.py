@@ -6,6 +6,7 @@ code, carrying the library's error text.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libpccl_hip.so")
@@ -60,37 +61,11 @@ class OpDesc(ctypes.Structure):
     ]
 
 
-class FoldNormDesc(ctypes.Structure):
-    """struct pccl_fold_norm_desc"""
-    _fields_ = [
-        ("dtype", ctypes.c_int), ("param_dtype", ctypes.c_int), ("post_kind", ctypes.c_int), ("pre_kind", ctypes.c_int),
-        ("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
-        ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float),
-        ("n_in", ctypes.c_int), ("n_out", ctypes.c_int), ("reserved", ctypes.c_int),
-        ("rows", ctypes.c_long), ("width", ctypes.c_long),
-        ("post_weight", ctypes.c_void_p), ("post_bias", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p), ("pre_bias", ctypes.c_void_p),
-        ("gate", ctypes.c_void_p), ("gate_stride", ctypes.c_long), ("gate_rows", ctypes.c_long),
-        ("ins", ctypes.c_void_p * MAX_INPUTS), ("in_stride", ctypes.c_long),
-        ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_long),
-        ("residual_out", ctypes.c_void_p), ("residual_out_stride", ctypes.c_long),
-        ("folded", ctypes.c_void_p), ("folded_stride", ctypes.c_long),
-        ("outs", ctypes.c_void_p * MAX_OUTPUTS), ("out_stride", ctypes.c_long),
-    ]
-
-
-class FoldNormGrads(ctypes.Structure):
-    """struct pccl_fold_norm_grads"""
-    _fields_ = [
-        ("grad_outs", ctypes.c_void_p * MAX_OUTPUTS), ("grad_out_stride", ctypes.c_long),
-        ("grad_residual_out", ctypes.c_void_p), ("grad_residual_out_stride", ctypes.c_long),
-        ("grad_ins", ctypes.c_void_p * MAX_INPUTS), ("n_grad_in", ctypes.c_int), ("reserved", ctypes.c_int),
-        ("grad_in_stride", ctypes.c_long),
-        ("grad_residual", ctypes.c_void_p), ("grad_residual_stride", ctypes.c_long),
-        ("grad_gate", ctypes.c_void_p), ("grad_gate_stride", ctypes.c_long),
-        ("grad_post_weight", ctypes.c_void_p), ("grad_post_bias", ctypes.c_void_p),
-        ("grad_pre_weight", ctypes.c_void_p), ("grad_pre_bias", ctypes.c_void_p),
-        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_long),
-    ]
+# struct pccl_fold_norm_desc and struct pccl_fold_norm_grads, packed in one go for each call (field by field through ctypes costs as
+# much as the launch): kinds and scales, n_in, n_out, rows, width; weights and biases; gate; ins; residual; residual_out; folded; outs
+_FOLD_NORM_DESC = struct.Struct("@4i5f3i2l 4P P2l 8Pl Pl Pl Pl 8Pl")
+# grad_outs; grad_residual_out; grad_ins, n_grad_in; grad_residual; grad_gate; gradients of weights and biases; workspace
+_FOLD_NORM_GRADS = struct.Struct("@8Pl Pl 8P2il Pl Pl 4P Pl")
 
 
 class CacheDesc(ctypes.Structure):
@@ -125,8 +100,8 @@ def lib():
         L.pccl_hip_free.argtypes = [vp]
         L.pccl_hip_reduce_copy.argtypes = [ci, ci, ctypes.POINTER(vp), ci, ctypes.POINTER(vp), ci, cl, vp]
         L.pccl_hip_accumulate.argtypes = [ci, ci, vp, ctypes.POINTER(vp), ci, cl, vp]
-        L.pccl_hip_fold_norm.argtypes = [ctypes.POINTER(FoldNormDesc), vp]
-        L.pccl_hip_fold_norm_backward.argtypes = [ctypes.POINTER(FoldNormDesc), ctypes.POINTER(FoldNormGrads), vp]
+        L.pccl_hip_fold_norm.argtypes = [vp, vp]
+        L.pccl_hip_fold_norm_backward.argtypes = [vp, vp, vp]
         L.pccl_hip_fold_norm_workspace.argtypes = [cl, cl, cl, ctypes.POINTER(cl)]
         L.pccl_hip_cache_write.argtypes = [ctypes.POINTER(CacheDesc), ci, ctypes.POINTER(vp), cl, cl, vp, cl, vp]
         L.pccl_hip_cache_read.argtypes = [ctypes.POINTER(CacheDesc), ci, ctypes.POINTER(vp), cl, cl, cl, vp, cl, vp, vp, ci, cl, vp]
@@ -243,18 +218,44 @@ def accumulate(dtype, compute, src, outs, count, stream=None):
                                      len(outs), count, ctypes.c_void_p(_addr(stream))))
 
 
+_ZEROS = [0] * 8
+
+
+def _at(x):
+    """Address of an operand, 0 for none."""
+    if x is None:
+        return 0
+    if type(x) is int:
+        return x
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return int(x)
+
+
 def _many(x, most, what):
-    """A list of operands, its length checked in front of the fixed array that it goes to."""
+    """Addresses of a list of operands, padded to the fixed array that they go to."""
     if len(x) > most:
         raise PcclError(ERR_INVALID_ARG, "%d %s, at most %d" % (len(x), what, most))
-    return [_addr(t) for t in x]
+    try:
+        at = [t.data_ptr() for t in x]  # (all of them tensors: half the time of asking each)
+    except AttributeError:
+        at = [_at(t) for t in x]
+    return at + _ZEROS[:most - len(x)]
 
 
 def _index(x, itemsize, count, what):
     """Address of a device array of whole numbers; of one that can tell its size (a torch tensor), the size is checked."""
-    if x is not None and hasattr(x, "element_size") and (x.element_size() != itemsize or x.numel() < count):
+    if x is not None and type(x) is not int and hasattr(x, "element_size") and (x.element_size() != itemsize or x.numel() < count):
         raise PcclError(ERR_INVALID_ARG, "%s: %d entries of %d bytes, %d of %d are needed" % (what, x.numel(), x.element_size(), count, itemsize))
-    return _addr(x)
+    return _at(x)
+
+
+def _packed(layout, *values):
+    try:
+        return layout.pack(*values)
+    except struct.error as e:  # a number that its field cannot hold
+        raise PcclError(ERR_INVALID_ARG, str(e)) from None
 
 
 class FoldNorm:
@@ -269,41 +270,28 @@ class FoldNorm:
 
     def __init__(self, dtype, width, post="none", pre="rms", param_dtype=None, post_weight=None, post_bias=None, pre_weight=None,
                  pre_bias=None, post_eps=1e-6, pre_eps=1e-6, weight_offset=0.0, residual_scale=1.0, block_scale=1.0):
-        self._keep = (post_weight, post_bias, pre_weight, pre_bias)
         self.width = width
-        d = self._desc = FoldNormDesc()
-        d.dtype = _code(DTYPES, dtype)
-        d.param_dtype = d.dtype if param_dtype is None else _code(DTYPES, param_dtype)
-        d.post_kind, d.pre_kind = _code(NORMS, post), _code(NORMS, pre)
-        d.post_eps, d.pre_eps, d.weight_offset = post_eps, pre_eps, weight_offset
-        d.residual_scale, d.block_scale = residual_scale, block_scale
-        d.width = width
-        d.post_weight, d.post_bias, d.pre_weight, d.pre_bias = (_addr(x) for x in self._keep)
+        self._params = (post_weight, post_bias, pre_weight, pre_bias)
+        dtype = _code(DTYPES, dtype)
+        self._settings = (dtype, dtype if param_dtype is None else _code(DTYPES, param_dtype), _code(NORMS, post), _code(NORMS, pre),
+                          *(ctypes.c_float(x).value for x in (post_eps, pre_eps, weight_offset, residual_scale, block_scale)))
 
-    def _call(self, ins, rows, gate, gate_rows, gate_stride, in_stride):
-        d = FoldNormDesc.from_buffer_copy(self._desc)
-        at = _many(ins, MAX_INPUTS, "inputs")
-        d.ins[:len(at)] = at
-        d.n_in, d.rows = len(at), rows
-        d.in_stride = self.width if in_stride is None else in_stride
-        if gate is not None:
-            d.gate, d.gate_rows = _addr(gate), gate_rows
-            d.gate_stride = self.width if gate_stride is None else gate_stride
-        return d
+    def _desc(self, ins, n_out, rows, gate, gate_rows, gate_stride, in_stride, residual, residual_stride, residual_out, residual_out_stride,
+              folded, folded_stride, outs, out_stride):
+        w = self.width
+        return _packed(_FOLD_NORM_DESC, *self._settings, len(ins), n_out, 0, rows, w, *[_at(x) for x in self._params],
+                       _at(gate), w if gate_stride is None else gate_stride, gate_rows, *_many(ins, MAX_INPUTS, "inputs"),
+                       w if in_stride is None else in_stride, _at(residual), w if residual_stride is None else residual_stride,
+                       _at(residual_out), w if residual_out_stride is None else residual_out_stride, _at(folded),
+                       w if folded_stride is None else folded_stride, *_many(outs, MAX_OUTPUTS, "outputs"), w if out_stride is None else out_stride)
 
     def forward(self, ins, outs, rows, residual=None, residual_out=None, folded=None, gate=None, gate_rows=0, stream=None,
                 in_stride=None, residual_stride=None, residual_out_stride=None, folded_stride=None, gate_stride=None, out_stride=None):
         """h to every buffer of `outs` (none: h is not computed), r to `residual_out`, y to `folded`, where given.  The gate
         has one row for every `gate_rows` rows.  Strides in elements from row to row, by default the width."""
-        w = self.width
-        d = self._call(ins, rows, gate, gate_rows, gate_stride, in_stride)
-        at = _many(outs, MAX_OUTPUTS, "outputs")
-        d.outs[:len(at)] = at
-        d.n_out, d.out_stride = len(at), w if out_stride is None else out_stride
-        d.residual, d.residual_stride = _addr(residual), w if residual_stride is None else residual_stride
-        d.residual_out, d.residual_out_stride = _addr(residual_out), w if residual_out_stride is None else residual_out_stride
-        d.folded, d.folded_stride = _addr(folded), w if folded_stride is None else folded_stride
-        _check(lib().pccl_hip_fold_norm(ctypes.byref(d), _addr(stream)))
+        d = self._desc(ins, len(outs), rows, gate, gate_rows, gate_stride, in_stride, residual, residual_stride, residual_out,
+                       residual_out_stride, folded, folded_stride, outs, out_stride)
+        _check(lib().pccl_hip_fold_norm(d, _at(stream)))
 
     def workspace_bytes(self, rows, gate_rows=0):
         """Bytes of workspace that backward needs for this many rows (gate_rows = 0: no gate)."""
@@ -321,26 +309,17 @@ class FoldNorm:
         parameters.  workspace: a buffer of workspace_bytes(rows, gate_rows), its size taken from the buffer where it can
         tell (a torch tensor), else from the argument."""
         w = self.width
-        d = self._call(ins, rows, gate, gate_rows, gate_stride, in_stride)
-        d.residual_out, d.residual_out_stride = _addr(residual_out), w if residual_out_stride is None else residual_out_stride
-        g = FoldNormGrads()
-        at = _many(grad_outs, MAX_OUTPUTS, "gradients of the outputs")
-        g.grad_outs[:len(at)] = at
-        d.n_out, g.grad_out_stride = len(at), w if grad_out_stride is None else grad_out_stride
-        at = _many(grad_ins, MAX_INPUTS, "gradients of the inputs")
-        g.grad_ins[:len(at)] = at
-        g.n_grad_in, g.grad_in_stride = len(at), w if grad_in_stride is None else grad_in_stride
-        g.grad_residual_out = _addr(grad_residual_out)
-        g.grad_residual_out_stride = w if grad_residual_out_stride is None else grad_residual_out_stride
-        g.grad_residual, g.grad_residual_stride = _addr(grad_residual), w if grad_residual_stride is None else grad_residual_stride
-        g.grad_gate, g.grad_gate_stride = _addr(grad_gate), w if grad_gate_stride is None else grad_gate_stride
-        g.grad_post_weight, g.grad_post_bias = _addr(grad_post_weight), _addr(grad_post_bias)
-        g.grad_pre_weight, g.grad_pre_bias = _addr(grad_pre_weight), _addr(grad_pre_bias)
-        if workspace is not None:
-            if workspace_bytes is None:
-                workspace_bytes = workspace.numel() * workspace.element_size()
-            g.workspace, g.workspace_bytes = _addr(workspace), workspace_bytes
-        _check(lib().pccl_hip_fold_norm_backward(ctypes.byref(d), ctypes.byref(g), _addr(stream)))
+        d = self._desc(ins, len(grad_outs), rows, gate, gate_rows, gate_stride, in_stride, None, None, residual_out, residual_out_stride, None, None,
+                       (), None)
+        if workspace is not None and workspace_bytes is None:
+            workspace_bytes = workspace.numel() * workspace.element_size()
+        g = _packed(_FOLD_NORM_GRADS, *_many(grad_outs, MAX_OUTPUTS, "gradients of the outputs"), w if grad_out_stride is None else grad_out_stride,
+                    _at(grad_residual_out), w if grad_residual_out_stride is None else grad_residual_out_stride,
+                    *_many(grad_ins, MAX_INPUTS, "gradients of the inputs"), len(grad_ins), 0, w if grad_in_stride is None else grad_in_stride,
+                    _at(grad_residual), w if grad_residual_stride is None else grad_residual_stride,
+                    _at(grad_gate), w if grad_gate_stride is None else grad_gate_stride, _at(grad_post_weight), _at(grad_post_bias),
+                    _at(grad_pre_weight), _at(grad_pre_bias), _at(workspace), workspace_bytes or 0)
+        _check(lib().pccl_hip_fold_norm_backward(d, g, _at(stream)))
 
 
 class Cache:
@@ -354,11 +333,12 @@ class Cache:
         d = self._desc = CacheDesc()
         d.format = _code(CACHE_FORMATS, fmt)
         d.heads, d.head_dim, d.page_tokens, d.n_pages = heads, head_dim, page_tokens, n_pages
-        codes, scales = _many(codes, CACHE_MAX_TENSORS, "tensors of codes"), _many(scales, CACHE_MAX_TENSORS, "tensors of scales")
         if len(codes) != len(scales):
             raise PcclError(ERR_INVALID_ARG, "%d tensors of codes, %d of scales" % (len(codes), len(scales)))
+        d.codes[:] = _many(codes, CACHE_MAX_TENSORS, "tensors of codes")
+        d.scales[:] = _many(scales, CACHE_MAX_TENSORS, "tensors of scales")
         d.n_tensors = self.n_tensors = len(codes)
-        d.codes[:len(codes)], d.scales[:len(scales)] = codes, scales
+        self._ref, self._array = ctypes.byref(d), ctypes.c_void_p * self.n_tensors  # (the description is only read from here on)
         row, blocks = self.row_bytes(fmt, head_dim)
         d.code_page, d.code_token, d.code_head = code_strides or (page_tokens * heads * row, heads * row, row)
         d.scale_page, d.scale_token, d.scale_head = scale_strides or (page_tokens * heads * blocks, heads * blocks, blocks)
@@ -372,7 +352,7 @@ class Cache:
     def _operands(self, x, what):
         if len(x) != self.n_tensors:
             raise PcclError(ERR_INVALID_ARG, "%d %s for %d tensors" % (len(x), what, self.n_tensors))
-        return (ctypes.c_void_p * len(x))(*[_addr(t) for t in x])
+        return self._array(*[_at(t) for t in x])
 
     def write(self, dtype, srcs, slots, tokens, stream=None, token_stride=None, head_stride=None):
         """Codes `tokens` rows of heads x head_dim elements of every source into slots[i] = page * page_tokens + token of the page
@@ -381,8 +361,8 @@ class Cache:
         srcs = self._operands(srcs, "sources")
         head_stride = self.head_dim if head_stride is None else head_stride
         token_stride = self.heads * self.head_dim if token_stride is None else token_stride
-        _check(lib().pccl_hip_cache_write(ctypes.byref(self._desc), _code(DTYPES, dtype), srcs, token_stride, head_stride,
-                                          _index(slots, 8, tokens, "slots"), tokens, _addr(stream)))
+        _check(lib().pccl_hip_cache_write(self._ref, _code(DTYPES, dtype), srcs, token_stride, head_stride,
+                                          _index(slots, 8, tokens, "slots"), tokens, _at(stream)))
 
     def read(self, dtype, outs, page_table, lengths, n_seq, max_len, row_start=None, out_rows=None, table_stride=None, stream=None,
              token_stride=None, head_stride=None):
@@ -399,10 +379,10 @@ class Cache:
             if row_start is not None:
                 raise PcclError(ERR_INVALID_ARG, "row_start without out_rows")
             out_rows = n_seq * max_len
-        _check(lib().pccl_hip_cache_read(ctypes.byref(self._desc), _code(DTYPES, dtype), outs, token_stride, head_stride, out_rows,
+        _check(lib().pccl_hip_cache_read(self._ref, _code(DTYPES, dtype), outs, token_stride, head_stride, out_rows,
                                          _index(page_table, 4, n_seq * table_stride, "page_table"), table_stride,
                                          _index(lengths, 4, n_seq, "lengths"), _index(row_start, 8, n_seq, "row_start"), n_seq, max_len,
-                                         _addr(stream)))
+                                         _at(stream)))
 
 
 def _op_descs(ops):
