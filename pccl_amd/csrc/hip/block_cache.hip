@@ -330,13 +330,15 @@ struct Place {
   int n, first;           // elements inside the head, the first of them
   long code, scale, row;  // bytes behind the token's start
 };
-template <class L, int PARTS>
+template <class L, int PARTS, int REPEAT>
 __device__ __forceinline__ Place place_of(const CacheArgs &a, unsigned chunk, int part) {
   Place p;
   const unsigned lane = threadIdx.x % kWave;
   p.token = PARTS ? 0 : a.token_lanes.divide(lane);
-  const unsigned r = PARTS ? (chunk * PARTS + part) * kWave + lane : lane - p.token * a.token_lanes.d;
-  p.on = PARTS ? r < a.token_lanes.d : p.token < a.group;
+  unsigned r = PARTS ? (chunk * PARTS + part) * kWave + lane : lane - p.token * a.token_lanes.d;
+  p.on = PARTS ? (chunk * PARTS + part) * kWave < a.token_lanes.d : p.token < a.group;
+  // lanes behind the token's last do what its last block's (or last) lanes do, to the same bytes: the wavefront stays whole
+  if (PARTS && r >= a.token_lanes.d) r = a.token_lanes.d - REPEAT + r % REPEAT;
   const unsigned head = a.head_lanes.divide(r);
   p.first = (int)(r - head * a.head_lanes.d) * L::kElems;
   p.n = min(max(a.head_dim - p.first, 0), L::kElems);
@@ -348,9 +350,11 @@ __device__ __forceinline__ Place place_of(const CacheArgs &a, unsigned chunk, in
 
 __device__ __forceinline__ unsigned long times(unsigned a, unsigned b) { return (unsigned long)a * b; }
 
-// Whether every lane of the wavefront has a whole piece in every part.  Then, and if every token of the wavefront is to be worked on, it
-// goes through code without a branch: the scalar unit, one instruction a clock for a compute unit's 32 wavefronts, is what the
-// masks of the general form keep busy (4-bit read of 131072 tokens x 8 x 128 x 2: 143 -> 117 us).
+// How much of a wavefront's work may be missing.  kAny: tokens, lanes, the ends of pieces.  kEven: heads are whole pieces, so a lane has
+// its piece or nothing, under one mask.  kWhole: every lane has a piece of every token; no mask and no branch.  The scalar unit, one
+// instruction a clock for a compute unit's 32 wavefronts, is what the masks of the general form keep busy (4-bit read of
+// 131072 tokens x 8 x 128 x 2: 143 us without kWhole, 120 with it).
+constexpr int kAny = 0, kEven = 1, kWhole = 2;
 template <class L, int PARTS>
 __device__ __forceinline__ bool all_whole(const Place (&p)[PARTS]) {
   bool whole = true;
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
   char *codes = a.codes[blockIdx.y], *scales = a.scales[blockIdx.y];
   Place p[kParts];
 #pragma unroll
-  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS>(a, chunk, h);
+  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS, L::kBlockLanes>(a, chunk, h);
   unsigned long slot[TIMES];
   u32x4 v[TIMES][kParts];
 #pragma unroll
@@ -390,14 +394,20 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
     if (!there) slot[t] = ~0ul;
   }
   const bool long_head = a.head_dim >= L::kElems;
-  auto work = [&](auto whole) {
-    constexpr bool kWhole = decltype(whole)::value;
+  auto work = [&](auto level) {
+    constexpr int kLevel = decltype(level)::value;
 #pragma unroll
     for (int t = 0; t < TIMES; ++t)
 #pragma unroll
-      for (int h = 0; h < kParts; ++h)
-        if (kWhole || (slot[t] < a.n_slots && p[h].on))
-          v[t][h] = L::template load<STREAM>(src + times(token0 + t * a.group + p[0].token, a.src_token) + p[h].row, kWhole ? L::kElems : p[h].n, long_head);
+      for (int h = 0; h < kParts; ++h) {
+        const char *at = src + times(token0 + t * a.group + p[0].token, a.src_token) + p[h].row;
+        if constexpr (kLevel == kWhole) {
+          v[t][h] = L::template load<STREAM>(at, L::kElems, true);
+        } else {
+          if (kLevel == kEven) v[t][h] = u32x4{0, 0, 0, 0};
+          if (slot[t] < a.n_slots && p[h].on && (kLevel == kAny || p[h].n)) v[t][h] = L::template load<STREAM>(at, kLevel == kEven ? L::kElems : p[h].n, long_head);
+        }
+      }
 #pragma unroll
     for (int t = 0; t < TIMES; ++t) {
       const unsigned page = a.page_tokens.divide((unsigned)slot[t]), token = (unsigned)slot[t] - page * a.page_tokens.d;
@@ -405,20 +415,28 @@ __global__ void __launch_bounds__(kBlock) cache_write_kernel(const WriteArgs a) 
       char *scale_to = scales + (times(page, a.scale_page) + times(token, a.scale_token));
 #pragma unroll
       for (int h = 0; h < kParts; ++h) {
-        if (!kWhole && (slot[t] >= a.n_slots || !p[h].on)) continue;  // whole blocks
+        const bool there = slot[t] < a.n_slots && p[h].on;  // the same for a block's lanes
+        if (kLevel == kAny && !there) continue;
         const unsigned s = scale_of<CacheFormat<FMT>>(block_max<L::kBlockLanes>(most_of<DT>(v[t][h])));
-        L::store_codes(to + p[h].code, kWhole ? L::kElems : p[h].n, L::encode(v[t][h], s));
-        if (p[h].first % PCCL_CACHE_BLOCK == 0) scale_to[p[h].scale] = (char)s;
+        const typename L::Codes c = L::encode(v[t][h], s);
+        if (kLevel != kEven || (there && p[h].n)) {
+          L::store_codes(to + p[h].code, kLevel == kAny ? p[h].n : L::kElems, c);
+          if (p[h].first % PCCL_CACHE_BLOCK == 0) scale_to[p[h].scale] = (char)s;
+        }
       }
     }
   };
+  typedef std::integral_constant<int, kAny> Any;
+  typedef std::integral_constant<int, kEven> Even;
+  typedef std::integral_constant<int, kWhole> Whole;
+  if (a.head_dim % L::kElems != 0) return work(Any{});
   if constexpr (PARTS != 0) {
     bool all = true;  // (on the scalar unit)
 #pragma unroll
     for (int t = 0; t < TIMES; ++t) all = all && slot[t] < a.n_slots;
-    if (all && all_whole<L>(p)) return work(std::true_type{});
+    if (all && all_whole<L>(p)) return work(Whole{});
   }
-  work(std::false_type{});
+  work(Even{});
 }
 
 struct ReadArgs : CacheArgs {
@@ -442,7 +460,7 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
   if ((long)token0 >= a.max_len) return;
   Place p[kParts];
 #pragma unroll
-  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS>(a, chunk, h);
+  for (int h = 0; h < kParts; ++h) p[h] = place_of<L, PARTS, 1>(a, chunk, h);
   // Table entries, length and first row are asked for together (an entry that is not the sequence's is inside the table all the
   // same): what a wavefront waits for is one chain of two loads.
   const int *table = a.page_table + seq * a.table_stride;
@@ -467,8 +485,8 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
     named[t] = named[t] && (long)pos < length && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows && page[t] < (unsigned long)a.n_pages;
   }
   const bool long_head = a.head_dim >= L::kElems;
-  auto work = [&](auto whole) {
-    constexpr bool kWhole = decltype(whole)::value;
+  auto work = [&](auto level) {
+    constexpr int kLevel = decltype(level)::value;
 #pragma unroll
     for (int t = 0; t < TIMES; ++t) {
       const unsigned pos = (unsigned)token0 + t * a.group + p[0].token, token = pos - a.page_tokens.divide(pos) * a.page_tokens.d;
@@ -476,9 +494,9 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
       const char *scale_from = scales + (times((unsigned)page[t], a.scale_page) + times(token, a.scale_token));
 #pragma unroll
       for (int h = 0; h < kParts; ++h) {
-        if (!kWhole && (!named[t] || !p[h].on)) continue;
+        if (kLevel != kWhole && !(named[t] && p[h].on)) continue;
         s[t][h] = (unsigned char)scale_from[p[h].scale];
-        c[t][h] = L::load_codes(from + p[h].code, kWhole ? L::kElems : p[h].n, long_head);
+        c[t][h] = L::load_codes(from + p[h].code, kLevel == kAny ? p[h].n : L::kElems, long_head);
       }
     }
 #pragma unroll
@@ -487,16 +505,20 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
       char *to = out + times((unsigned)(first_row + pos), a.out_token);
 #pragma unroll
       for (int h = 0; h < kParts; ++h)
-        if (kWhole || (named[t] && p[h].on)) L::store(to + p[h].row, kWhole ? L::kElems : p[h].n, L::decode(c[t][h], s[t][h]));
+        if (kLevel == kWhole || (named[t] && p[h].on)) L::store(to + p[h].row, kLevel == kAny ? p[h].n : L::kElems, L::decode(c[t][h], s[t][h]));
     }
   };
+  typedef std::integral_constant<int, kAny> Any;
+  typedef std::integral_constant<int, kEven> Even;
+  typedef std::integral_constant<int, kWhole> Whole;
+  if (a.head_dim % L::kElems != 0) return work(Any{});
   if constexpr (PARTS != 0) {
     bool all = true;  // (on the scalar unit)
 #pragma unroll
     for (int t = 0; t < TIMES; ++t) all = all && named[t];
-    if (all && all_whole<L>(p)) return work(std::true_type{});
+    if (all && all_whole<L>(p)) return work(Whole{});
   }
-  work(std::false_type{});
+  work(Even{});
 }
 
 }  // namespace pccl_dev
