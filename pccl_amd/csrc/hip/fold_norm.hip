@@ -100,7 +100,7 @@ void fill(const pccl_fold_norm_desc *d, const Checker &c, NormArgs *a) {
   a->post_bias = (const char *)d->post_bias;
   a->pre_weight = (const char *)d->pre_weight;
   a->pre_bias = (const char *)d->pre_bias;
-  a->gate = (const char *)d->gate;
+  a->gate = d->rows ? (const char *)d->gate : nullptr;  // (without rows it has none either)
   a->gate_bytes = d->gate_stride * c.ps;
   a->gate_rows = (unsigned)(d->gate ? std::min(d->gate_rows, std::max(1l, d->rows)) : std::max(1l, d->rows));
   for (int k = 0; k < d->n_in; ++k) a->ins[k] = (const char *)d->ins[k];
@@ -264,7 +264,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   a.n_teams = cut.n_teams;
   a.sums = (float *)g->workspace;
   a.gate_sums = joined_gate ? (float *)((char *)g->workspace + (any ? sums_bytes(cut, d->width) : 0)) : nullptr;
-  a.grad_gate = d->rows ? (char *)g->grad_gate : nullptr;  // (no rows: no gate row either)
+  a.grad_gate = d->rows ? (char *)g->grad_gate : nullptr;
   a.grad_gate_bytes = g->grad_gate_stride * c.ps;
   for (int k = 0; k < 4; ++k) a.want_sums[k] = to[k] != nullptr;
   // beyond the Infinity Cache (bf16 16384 x 8192 306 -> 281 us, 32768 x 1024 88 -> 83; inside: 8192 x 2048 with a gate a row 84.5 -> 86)

@@ -411,14 +411,14 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
       if (pre) {
         // dr += rstd * (d - rhat * mean(d * rhat) - mean(d)), d = dh * w
         const float rstd = one_over_spread(q[1], per_width, a->pre_eps);
-        const float along = -(rstd * rstd * rstd) * (q[2] * per_width);
+        const float along = -rstd * (q[2] * per_width);  // (no power of rstd on its own: with a tiny eps that could pass the largest binary32)
         float w[kWide ? E : 1];
         if constexpr (kWide) get_wpre(w);
         const auto &wpre = [&]() -> const float (&)[E] { if constexpr (kWide) return w; else return wpre_kept; }();
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          dr[i] = __builtin_fmaf(dh[i] * wpre[i], rstd, __builtin_fmaf(r[i], along, dr[i]));
           r[i] *= rstd;
+          dr[i] = __builtin_fmaf(rstd, __builtin_fmaf(r[i], along, dh[i] * wpre[i]), dr[i]);
         }
         p1.add(dh, r);
         if (pre_layer) {

@@ -167,6 +167,147 @@ def test_zero_constant_and_infinite_rows(hip):
             within(out[fine], (want[0][fine], want[1][fine]), dtype, "%s %s" % (kinds, dtype))
 
 
+@pytest.mark.parametrize("width", [40, 700, 9000])
+def test_tiny_eps(hip, width):
+    """eps near the smallest it may be: rows of zeros have gradients of zero and 1 / sqrt(eps), not NaN."""
+    import torch
+    n = 5
+    gen = torch.Generator().manual_seed(6)
+    p = params(torch, gen, width, "f32")
+    p["post_eps"] = p["pre_eps"] = 1e-37
+    L = layer_of(hip, "f32", width, p)
+    y, r, dh = (rows(torch, gen, "f32", n, width) for _ in range(3))
+    y[1], r[2], r[3], dh[2], dh[3] = 0, 0, 0, 0, dh[3] * 1e-20
+    new = lambda: torch.zeros(n, width, device="cuda")  # noqa: E731
+    dy, dx, w1, w2 = new(), new(), torch.zeros(width, device="cuda"), torch.zeros(width, device="cuda")
+    ws = torch.zeros(L.workspace_bytes(n), dtype=torch.uint8, device="cuda")
+    L.backward([y.cuda()], [dh.cuda()], [dy], n, residual_out=r.cuda(), grad_residual=dx, grad_post_weight=w1, grad_pre_weight=w2, workspace=ws)
+    torch.cuda.synchronize()
+    p = dict(p, post_eps=float(torch.tensor(1e-37)), pre_eps=float(torch.tensor(1e-37)))
+    want = ref.backward(y.double()[None], r.double(), dh.double()[None], torch.zeros(n, width, dtype=torch.float64), None, 0, p)
+    within(dx[:3], tuple(v[:3] for v in want["grad_residual"]), "f32", "dx")
+    assert bool((dx[2] == 0).all()) and bool(torch.isfinite(dx).all())
+    keep = [0, 2, 4]  # (the row of zeros in y: its gradient is past 10^18 times the others')
+    within(dy[keep], tuple(v[keep] for v in want["grad_ins"]), "f32", "dy")
+    assert not bool(torch.isnan(dy).any()) and not bool(torch.isnan(w1).any()) and not bool(torch.isnan(w2).any())
+
+
+def test_no_rows(hip):
+    """Gradients of parameters over no rows are zero; nothing of rows or gate is touched."""
+    import torch
+    for width in (3, 700, 9000):
+        gen = torch.Generator().manual_seed(6)
+        p = params(torch, gen, width, "f32", "layer", "layer", biases=True)
+        L = layer_of(hip, "f32", width, p)
+        w = [torch.full((width,), 7.0, device="cuda") for _ in range(4)]
+        ws = torch.full((L.workspace_bytes(0, 3),), 0x5A, dtype=torch.uint8, device="cuda")
+        L.backward([None], [None], [None], 0, gate=0x1000, gate_rows=3, grad_gate=0x2000, grad_post_weight=w[0], grad_post_bias=w[1], grad_pre_weight=w[2],
+                   grad_pre_bias=w[3], workspace=ws)
+        L.forward([None], [None], 0, gate=0x1000, gate_rows=3)
+        torch.cuda.synchronize()
+        assert all(bool((v == 0).all()) for v in w)
+
+
+@pytest.mark.parametrize("n,width,gate_rows,biases", [(300, 8192, 1, False), (300, 8192, 1, True), (300, 8200, 1, False), (290, 9000, 1, True), (4500, 40, 1, True),
+                                                      (2100, 600, 1, False), (101, 600, 100, True), (5000, 64, 2, True), (700, 4100, 2, True)])
+def test_more_gate_rows_than_teams(hip, n, width, gate_rows, biases):
+    """A team then goes through several gate rows and keeps its sums over them; and a last gate row of one row."""
+    import torch
+    gen = torch.Generator().manual_seed(14)
+    p = params(torch, gen, width, "bf16", "rms", "layer", biases=biases)
+    L = layer_of(hip, "bf16", width, p)
+    groups = -(-n // gate_rows)
+    y, r, dh, dr = (rows(torch, gen, "bf16", n, width) for _ in range(4))
+    gate = rows(torch, gen, "bf16", groups, width)
+    want = ref.backward(y.double()[None], r.double(), dh.double()[None], dr.double(), gate.double(), gate_rows, p)
+    dy, dx, dg = torch.zeros_like(y, device="cuda"), torch.zeros_like(y, device="cuda"), torch.zeros_like(gate, device="cuda")
+    names = ["post_weight", "pre_weight"] + (["post_bias", "pre_bias"] if biases else [])
+    w = {k: torch.zeros(width, dtype=torch.bfloat16, device="cuda") for k in names}
+    ws = torch.full((L.workspace_bytes(n, gate_rows),), 0x5A, dtype=torch.uint8, device="cuda")
+    L.backward([y.cuda()], [dh.cuda()], [dy], n, residual_out=r.cuda(), grad_residual_out=dr.cuda(), grad_residual=dx, gate=gate.cuda(), gate_rows=gate_rows,
+               grad_gate=dg, workspace=ws, **{"grad_" + k: v for k, v in w.items()})
+    torch.cuda.synchronize()
+    within(dx, want["grad_residual"], "bf16", "dx")
+    within(dy, want["grad_ins"], "bf16", "dy")
+    within(dg, want["grad_gate"], "bf16", "gate")
+    for k in names:
+        within(w[k], want["grad_" + k], "bf16", k)
+
+
+@pytest.mark.parametrize("dtype,width,n_in,n_out", [("bf16", 4096, 4, 3), ("f32", 8192, 3, 2), ("f16", 12000, 8, 1), ("f32", 10000, 3, 1), ("bf16", 400, 5, 2)])
+def test_large_calls_give_the_bits_of_small_ones(hip, dtype, width, n_in, n_out):
+    """Beyond the Infinity Cache rows are read non-temporally, by instances of their own: the same rows in slices of less."""
+    import torch
+    size = 4 if dtype == "f32" else 2
+    n = (300 << 20) // (width * size * (n_in + n_out + 2)) + 7
+    gen = torch.Generator().manual_seed(15)
+    p = params(torch, gen, width, dtype, "layer", "rms", biases=True)
+    L = layer_of(hip, dtype, width, p)
+    t = ref.TYPES[dtype]
+    dev = torch.Generator(device="cuda").manual_seed(15)
+    make = lambda: torch.randn(n, width, device="cuda", generator=dev).to(t)  # noqa: E731
+    parts, x = [make() for _ in range(n_in)], make()
+    got = [torch.zeros_like(x) for _ in range(2 + n_out)]
+    want = [torch.zeros_like(x) for _ in range(2 + n_out)]
+    L.forward(parts, got[2:], n, residual=x, residual_out=got[0], folded=got[1])
+    step = n // 5 + 1
+    for lo in range(0, n, step):
+        cut = lambda v: v[lo:lo + step]  # noqa: E731
+        L.forward([cut(v) for v in parts], [cut(v) for v in want[2:]], cut(x).shape[0], residual=cut(x), residual_out=cut(want[0]), folded=cut(want[1]))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    # the backward pass reads four rows and writes two for each
+    n = min(n, (300 << 20) // (width * size * 6) + 7) if n * width * size * 5 > (300 << 20) else n
+    y, r, dh, dr = (v[:n] for v in (parts + [x, got[0], got[1]])[:4])
+    a, b = [torch.zeros_like(y) for _ in range(2)], [torch.zeros_like(y) for _ in range(2)]
+    L.backward([y], [dh], [a[0]], n, residual_out=r, grad_residual_out=dr, grad_residual=a[1])
+    step = n // 5 + 1
+    for lo in range(0, n, step):
+        cut = lambda v: v[lo:lo + step]  # noqa: E731
+        L.backward([cut(y)], [cut(dh)], [cut(b[0])], cut(y).shape[0], residual_out=cut(r), grad_residual_out=cut(dr), grad_residual=cut(b[1]))
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("fmt,dtype,heads,dim", [("f8e4m3", "bf16", 8, 128), ("f4e2m1", "f16", 1, 64), ("i8", "f32", 3, 80), ("f8e5m2", "bf16", 7, 61), ("f4e2m1", "bf16", 2, 33),
+                                                 ("i8", "f16", 9, 72), ("f8e4m3", "f32", 1, 20)])
+def test_large_cache_calls_give_the_bits_of_small_ones(hip, fmt, dtype, heads, dim):
+    """Large calls keep several tokens of a wavefront in flight and read their sources non-temporally, by instances of their own."""
+    import torch
+    t = ref.TYPES[dtype]
+    n = (100 << 20) // (heads * dim * (4 if dtype == "f32" else 2)) + 13
+    page = 48
+    pages = -(-n // page) + 1
+    row, blocks = hip.Cache.row_bytes(fmt, dim)
+    dev = torch.Generator(device="cuda").manual_seed(16)
+    x = (torch.randn(n, heads, dim, device="cuda", generator=dev) * torch.exp(2 * torch.randn(n, heads, 1, device="cuda", generator=dev))).to(t)
+    slots = torch.randperm(pages * page, device="cuda", generator=dev)[:n].clone()
+    slots[torch.rand(n, device="cuda", generator=dev) < 0.02] = -1
+    held = []
+    for step in (n, n // 400 + 1):
+        codes, scales = torch.zeros(pages, page, heads, row, dtype=torch.uint8, device="cuda"), torch.zeros(pages, page, heads, blocks, dtype=torch.uint8, device="cuda")
+        c = hip.Cache(fmt, heads, dim, page, pages, [codes], [scales])
+        for lo in range(0, n, step):
+            part = x[lo:lo + step]
+            c.write(dtype, [part], slots[lo:lo + step], part.shape[0])
+        held.append((codes, scales, c))
+    torch.cuda.synchronize()
+    assert torch.equal(held[0][0], held[1][0]) and torch.equal(held[0][1], held[1][1])
+    c = held[0][2]
+    table = torch.randperm(pages, device="cuda", generator=dev).int()
+    out, want = torch.full((pages * page, heads, dim), 3.0, dtype=t, device="cuda"), torch.full((pages * page, heads, dim), 3.0, dtype=t, device="cuda")
+    most = pages * page - 5
+    c.read(dtype, [out], table[None], torch.tensor([most], dtype=torch.int32, device="cuda"), 1, pages * page)
+    some = pages // 300 + 1
+    for lo in range(0, pages, some):
+        part = table[lo:lo + some].contiguous()
+        length = min(part.numel() * page, most - lo * page)
+        c.read(dtype, [want[lo * page:]], part[None], torch.tensor([length], dtype=torch.int32, device="cuda"), 1, part.numel() * page)
+    torch.cuda.synchronize()
+    assert torch.equal(out.view(torch.uint8), want.view(torch.uint8))
+
+
 def test_captured_and_replayed(hip):
     """Forward, backward, cache write and read recorded into a graph and replayed five times on new inputs, with eager calls and
     synchronizations between: every replay gives the bits of the eager call."""
