@@ -245,9 +245,12 @@ def _many(x, most, what):
 
 
 def _index(x, itemsize, count, what):
-    """Address of a device array of whole numbers; of one that can tell its size (a torch tensor), the size is checked."""
-    if x is not None and type(x) is not int and hasattr(x, "element_size") and (x.element_size() != itemsize or x.numel() < count):
-        raise PcclError(ERR_INVALID_ARG, "%s: %d entries of %d bytes, %d of %d are needed" % (what, x.numel(), x.element_size(), count, itemsize))
+    """Address of a device array of whole numbers; of one that can tell (a torch tensor), size and order are checked."""
+    if x is not None and type(x) is not int and hasattr(x, "element_size"):
+        if x.element_size() != itemsize or x.numel() < count:
+            raise PcclError(ERR_INVALID_ARG, "%s: %d entries of %d bytes, %d of %d are needed" % (what, x.numel(), x.element_size(), count, itemsize))
+        if not x.is_contiguous():  # (an expanded one has fewer entries in memory than it counts)
+            raise PcclError(ERR_INVALID_ARG, "%s: entries must lie side by side" % what)
     return _at(x)
 
 
@@ -356,7 +359,7 @@ class Cache:
 
     def write(self, dtype, srcs, slots, tokens, stream=None, token_stride=None, head_stride=None):
         """Codes `tokens` rows of heads x head_dim elements of every source into slots[i] = page * page_tokens + token of the page
-        (int64 on the device; a slot outside the cache: the row is left out).  The slots of one call must differ.  Strides in
+        (int64 on the device, side by side; a slot outside the cache: the row is left out).  The slots of one call must differ.  Strides in
         elements, by default those of a dense [tokens, heads, head_dim]."""
         srcs = self._operands(srcs, "sources")
         head_stride = self.head_dim if head_stride is None else head_stride
@@ -368,12 +371,14 @@ class Cache:
              token_stride=None, head_stride=None):
         """Token t < lengths[s] of sequence s, from page page_table[s][t // page_tokens], to row row_start[s] + t of every output (of
         `out_rows` rows), or without row_start to row s * max_len + t.  page_table, lengths (int32) and row_start (int64) are on
-        the device; table_stride, the entries of a sequence, is by default what a dense 2-d table says.  Rows that no token goes to
+        the device, their entries side by side; table_stride, the entries of a sequence, is by default what a dense 2-d table says.  Rows that no token goes to
         are left as they are."""
         outs = self._operands(outs, "outputs")
         head_stride = self.head_dim if head_stride is None else head_stride
         token_stride = self.heads * self.head_dim if token_stride is None else token_stride
         if table_stride is None:
+            if not hasattr(page_table, "shape"):
+                raise PcclError(ERR_INVALID_ARG, "table_stride is needed where the page table cannot tell it")
             table_stride = page_table.shape[-1]
         if out_rows is None:
             if row_start is not None:

@@ -148,6 +148,20 @@ def test_cache_index_arrays_that_tell_their_size():
     refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table, n, 2, 8, row_start=n.long())
 
 
+def test_cache_index_arrays_in_another_order():
+    import torch
+    c = cache()
+    table, n, rows = torch.zeros(4, 6, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), torch.zeros(8, dtype=torch.int64)
+    refused(hip.ERR_INVALID_ARG, c.write, "bf16", [A, A], rows[::2], 4)
+    refused(hip.ERR_INVALID_ARG, c.write, "bf16", [A, A], rows[:1].expand(4), 4)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table[:, :4], n, 4, 8)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table[:1].expand(4, 6), n, 4, 8)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table.t(), n, 4, 8)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table, n[::2], 4, 8)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], table, n, 4, 8, row_start=rows[::2], out_rows=32)
+    refused(hip.ERR_INVALID_ARG, c.read, "bf16", [A, A], A, A, 4, 8)
+
+
 def test_cache_read():
     c = cache()
     r = lambda outs=(A, A), table=A, lengths=A, n=1, most=8, stride=4, **kw: c.read(  # noqa: E731
