@@ -185,8 +185,8 @@ typedef struct pccl_fold_norm_desc {
   long out_stride;
 } pccl_fold_norm_desc;
 
-/* The forward pass.  One kernel launch on `stream`, which must belong to the current device; returns without
- * waiting.  An output may be the same buffer as an input (same address, same stride); other overlaps are undefined. */
+/* The forward pass.  One kernel launch (for every 2^21 rows) on `stream`, which must belong to the current device; returns
+ * without waiting.  An output may be the same buffer as an input (same address, same stride); other overlaps are undefined. */
 int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream);
 
 /* Gradients.  Of the forward's description the backward pass reads the norms, scales, parameters and gate,
@@ -262,8 +262,8 @@ typedef struct pccl_cache_desc {
 /* Codes `tokens` rows of heads x head_dim elements (f32, bf16 or f16; strides in elements) of every source and writes
  * row i to slot slots[i] = page * page_tokens + token of the page (device memory, read when the kernel runs).  A row whose slot is
  * below 0 or beyond the last page is neither read nor written.  Slots of one call must differ; a slot named twice holds
- * unspecified codes afterwards, all others are as they should be.  One kernel launch on `stream`, which must belong to the
- * current device; returns without waiting. */
+ * unspecified codes afterwards, all others are as they should be.  One kernel launch (more beyond millions of tokens) on `stream`,
+ * which must belong to the current device; returns without waiting. */
 int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const void *const *srcs, long src_token_stride, long src_head_stride,
                          const long *slots, long tokens, void *stream);
 

@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kBlock) cache_read_kernel(const ReadArgs a) {
 #pragma unroll
   for (int t = 0; t < TIMES; ++t) {
     const unsigned pos = (unsigned)token0 + t * a.group + p[0].token;
-    named[t] = named[t] && (long)pos < length && (unsigned long)(first_row + pos) < (unsigned long)a.out_rows && page[t] < (unsigned long)a.n_pages;
+    named[t] = named[t] && (long)pos < length && (unsigned long)first_row + pos < (unsigned long)a.out_rows && page[t] < (unsigned long)a.n_pages;
   }
   const bool long_head = a.head_dim >= L::kElems;
   auto work = [&](auto level) {
@@ -605,11 +605,7 @@ void with_types(int dtype, int format, F &&f) {
   else of_format(std::integral_constant<int, PCCL_F16>{});
 }
 
-#ifndef WT
-#define WT 2
-#define RT 4
-#endif
-constexpr int kWriteTimes = WT, kReadTimes = RT;  // groups of tokens that a wavefront has in flight where there are enough of them
+constexpr int kWriteTimes = 2, kReadTimes = 4;  // groups of tokens that a wavefront has in flight where there are enough of them
 
 // whether n wavefronts' worth of tokens, `times` of them to a wavefront, give every compute unit eight workgroups
 bool many(long n, int times) { return n >= (long)pccl_host::compute_units() * 8 * kWaves * times; }
@@ -663,7 +659,7 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
   a.src_token = (unsigned)(src_token_stride * es);
   a.row_head = src_head_stride * es;
   a.n_slots = (unsigned long)(c->n_pages * c->page_tokens);
-  const bool stream_in = (long)c->heads * c->head_dim * es * tokens * c->n_tensors >= (48l << 20);
+  const bool stream_in = (double)c->heads * c->head_dim * es * tokens * c->n_tensors >= (double)(48l << 20);  // (up to 2^68)
   const long most = launch_tokens(a);
   for (long lo = 0; lo < tokens; lo += most) {
     const long n = std::min(most, tokens - lo);

@@ -42,7 +42,7 @@ struct Checker {
   }
 };
 
-long gate_row_count(long rows, long gate_rows) { return (rows + gate_rows - 1) / gate_rows; }
+long gate_row_count(long rows, long gate_rows) { return rows / gate_rows + (rows % gate_rows != 0); }  // (gate_rows may be anything from 1)
 
 // What both directions look at.
 int check_desc(const pccl_fold_norm_desc *d, Checker *c) {
