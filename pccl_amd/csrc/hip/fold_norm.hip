@@ -15,9 +15,13 @@ namespace {
 // Rows of a launch: a grid times its lanes must fit 32 bits, 2^22 - 1 workgroups of 1024.
 constexpr unsigned kLaunchRows = 1u << 21;
 
-// A wavefront up to 512 elements (no barrier in its sums), beyond a workgroup of as many wavefronts as the width fills.
-NormShape shape_of(long width) {
-  const int elems = width <= 8192 ? 8 : 16;
+// One pack of 16 bytes a lane while a workgroup holds the row, else two (binary32 beyond 8192 columns: four): a wavefront where one is
+// enough (no barrier in its sums), beyond a workgroup of as many as the width fills.  (binary32 up to 4096 columns with one pack
+// and not two: forward 8192 x 2048 53 -> 48 us, 4096 x 4096 4 -> 2 95 -> 90; backward, where it is what leaves room for a row ahead,
+// 4985 x 1025 50 -> 41, 16384 x 1024 83 -> 80.  Without a row ahead the backward pass loses, 3000 x 4000 of two gradients 94 -> 97, and
+// with rows of 257 to 512 columns, where two packs still are one wavefront's, 50000 x 400 92 -> 97.)
+NormShape shape_of(long width, int dtype, bool one_pack) {
+  const int elems = dtype == PCCL_F32 && one_pack && width <= 4096 ? 4 : width <= 8192 ? 8 : 16;
   return {(int)((width + elems * kWave - 1) / (elems * kWave)) * kWave, elems};
 }
 
@@ -122,17 +126,26 @@ int launched(hipError_t e, const char *what) {
   return e == hipSuccess ? PCCL_OK : fail(PCCL_ERR_HIP, "%s launch failed: %s", what, hipGetErrorString(e));
 }
 
+// Shape of the backward pass.  `single`: one y and at most one gradient of h.
+NormShape backward_shape(long width, int dtype, bool single) { return shape_of(width, dtype, single && (width <= 4 * kWave || width > 8 * kWave)); }
+
 // How the backward pass cuts the rows (see BackwardArgs).
 struct Cut {
   unsigned groups, strips, n_strips, n_teams;
 };
 
 // Teams that fill the chip: enough for several wavefronts on every SIMD, few enough that writing and joining their sums
-// (4 rows of binary32 a team) stays small beside the rows themselves.
-Cut cut_of(long rows, long width, long gate_rows) {
-  const NormShape n = shape_of(width);
-  const long most = (long)pccl_host::compute_units() * (kMostLanes / n.lanes);
+// (4 rows of binary32 a team) stays small beside the rows themselves.  Twelve wavefronts a compute unit (or the team that
+// passes twelve) where teams have their next row on its way, sixteen where they wait for it: without a row ahead, and with
+// gate rows so short that a strip has none (`ahead` with 12 against 16: 8000 x 1536 bf16, 8 gate rows, 51 -> 48 us, 100000 x 200
+// f32 96 -> 88; 8192 x 2048 with a gate a row 65 -> 68, 4096 x 4096 of four gradients 89 -> 107).
+Cut cut_of(long rows, long width, long gate_rows, int dtype, bool single) {
+  const NormShape n = backward_shape(width, dtype, single);
+  const bool ahead = single && n.elems * pccl_host::pccl_dtype_bytes(dtype) == 16;
   const long per = gate_rows >= 1 ? std::min(gate_rows, std::max(1l, rows)) : std::max(1l, rows);
+  int teams = kMostLanes / n.lanes;
+  if (ahead && per >= 4) teams = std::min(teams, (12 * kWave + n.lanes - 1) / n.lanes);
+  const long most = (long)pccl_host::compute_units() * teams;
   Cut c;
   c.groups = (unsigned)std::max(1l, gate_row_count(rows, per));
   c.strips = (unsigned)std::max(1l, std::min(per, most / (long)c.groups));
@@ -173,7 +186,7 @@ extern "C" int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream) {
   a.folded_bytes = d->folded_stride * c.es;
   for (int j = 0; j < d->n_out; ++j) a.outs[j] = (char *)d->outs[j];
   a.out_bytes = d->out_stride * c.es;
-  const NormShape n = shape_of(d->width);
+  const NormShape n = shape_of(d->width, d->dtype, true);
   // many inputs beyond the Infinity Cache are read non-temporally (8 -> 8 bf16 at 2048 x 8192 122 -> 120 us, 8 -> 1 at 4096 x 4096 67 -> 64;
   // one or two lose: 1 -> 1 at 16384 x 8192 178 -> 184, and so does what is in that cache: f32 2 -> 2 at 4096 x 2048 38 -> 45)
   const bool stream_in = (d->n_in + d->n_out + 2) * d->rows * d->width * c.es > (256l << 20);
@@ -195,8 +208,12 @@ extern "C" int pccl_hip_fold_norm_workspace(long rows, long width, long gate_row
   if (rows < 0 || rows > 0x7fffffffl) return fail(PCCL_ERR_INVALID_ARG, "rows %ld outside [0, 2^31)", rows);
   if (width < 1 || width > PCCL_NORM_MAX_WIDTH) return fail(PCCL_ERR_INVALID_ARG, "width %ld outside [1, %d]", width, PCCL_NORM_MAX_WIDTH);
   if (gate_rows < 0) return fail(PCCL_ERR_INVALID_ARG, "gate_rows %ld < 0", gate_rows);
-  const Cut c = cut_of(rows, width, gate_rows);
-  *bytes = sums_bytes(c, width) + (gate_rows ? gate_sums_bytes(c, width) : 0);
+  for (int dtype : {PCCL_F32, PCCL_BF16}) {  // whichever type the rows have, and however many gradients there are
+    for (bool single : {false, true}) {
+      const Cut c = cut_of(rows, width, gate_rows, dtype, single);
+      *bytes = std::max(*bytes, sums_bytes(c, width) + (gate_rows ? gate_sums_bytes(c, width) : 0));
+    }
+  }
   return PCCL_OK;
 }
 
@@ -233,7 +250,9 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
     any = any || to[k];
   }
   if (c.rc != PCCL_OK) return c.rc;
-  const Cut cut = cut_of(d->rows, d->width, d->gate ? d->gate_rows : 0);
+  const bool single = d->n_in == 1 && d->n_out <= 1;
+  const NormShape shape = backward_shape(d->width, d->dtype, single);
+  const Cut cut = cut_of(d->rows, d->width, d->gate ? d->gate_rows : 0, d->dtype, single);
   const bool joined_gate = g->grad_gate && cut.strips > 1;
   const long need = (any ? sums_bytes(cut, d->width) : 0) + (joined_gate ? gate_sums_bytes(cut, d->width) : 0);
   if (need) {
@@ -271,7 +290,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   const bool stream_in = (4 + g->n_grad_in) * d->rows * d->width * c.es > (256l << 20);
   const bool bias = to[1] || to[3] || (g->grad_gate && d->post_bias);
   rc = launched(with_types(d->dtype, d->param_dtype, [&](auto t, auto p) {
-    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape_of(d->width), bias, stream_in, (hipStream_t)stream, a);
+    return launch_fold_norm_backward<decltype(t)::value, decltype(p)::value>(shape, single, bias, stream_in, (hipStream_t)stream, a);
   }), "fold_norm_backward");
   if (rc != PCCL_OK || !need) return rc;
 
@@ -284,7 +303,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
     if (to[k]) j.listed[j.n_listed++] = k;
   }
   j.width = (int)d->width;
-  j.n_partial = shape_of(d->width).workgroups(cut.n_teams);
+  j.n_partial = shape.workgroups(cut.n_teams);
   j.strips = cut.strips;
   j.grad_gate = a.grad_gate;
   j.grad_gate_bytes = a.grad_gate_bytes;

@@ -220,8 +220,9 @@ struct Columns {
 // so that a row costs one fused multiply-add a column for each, and gate and weight are met once a strip.
 //
 // One team's registers hold the row (packed), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, s1 and p1.
-// 16-bit rows of up to 8192 columns (E = 8) that are four streams (SINGLE: one y and at most one dh) have room for the row
-// after it, on its way; binary32 rows spilled with it (8192 x 2048 87 -> 84 us without).  s0 and p0 and the post norm's sums over a
+// Rows of one pack a lane (16-bit up to 8192 columns, binary32 up to 4096) that are four streams (SINGLE: one y and at most one dh) have
+// room for the row after it, on its way; binary32 with two packs spilled with it (8192 x 2048 87 -> 84 us without, 78 with one pack
+// and the row ahead).  s0 and p0 and the post norm's sums over a
 // team's strips stay in LDS.  Wider rows (E = 16) keep s1 and p1 there instead, the post norm's sums over strips go to the
 // workspace and back.
 // BIAS: some bias's gradient or a gate behind a biased norm is asked for (s0 and p0 are kept).
@@ -240,7 +241,7 @@ struct BackRow {
 };
 
 template <int DT, int E>
-constexpr bool row_ahead() { return DT != PCCL_F32 && E == 8; }
+constexpr bool row_ahead() { return E == RowType<DT>::kPack; }
 
 template <int DT, bool PF32, bool TEAM, int E, bool SINGLE, bool BIAS, bool STREAM>
 __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel(const BackwardArgs) {
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
   float wpre_kept[kWide ? 1 : E], ones[E];
   Columns<E, kWide> p1{{}, columns(0), (int)blockDim.x}, s1{{}, columns(1), (int)blockDim.x};
   Columns<E, !kWide> p0{{}, columns(2), (int)blockDim.x}, s0{{}, columns(3), (int)blockDim.x};                   // (BIAS)
-  Columns<E, true> post_sums{{}, columns(0), (int)blockDim.x}, post_bias_sums{{}, columns(1), (int)blockDim.x};  // (E = 8)
+  Columns<E, true> post_sums{{}, columns(0), (int)blockDim.x}, post_bias_sums{{}, columns(1), (int)blockDim.x};  // (E up to 8)
   p1.zero();
   if constexpr (BIAS) p0.zero();
 #pragma unroll
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
     if (a0->want_sums[3]) put(3, there, x_p0);
 }
 
-// Bytes of LDS for sums by column: with E = 8 the post norm's, with biases theirs, p0 and s0 too; with E = 16 p1 and s1.
+// Bytes of LDS for sums by column: with E up to 8 the post norm's, with biases theirs, p0 and s0 too; with E = 16 p1 and s1.
 inline unsigned backward_lds(int lanes_of_workgroup, int elems, bool bias) {
   return (unsigned)lanes_of_workgroup * elems * 4 * (elems > 8 ? 2 : bias ? 4 : 1);
 }
@@ -653,22 +654,26 @@ struct NormShape {
   unsigned workgroups(unsigned rows) const { return lanes == kWave ? (rows + kBlock / kWave - 1) / (kBlock / kWave) : rows; }
 };
 
-template <class F>
+template <int DT, class F>
 inline void with_norm_shape(NormShape n, F &&f) {
+  typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
   typedef std::integral_constant<int, 16> Sixteen;
+  if constexpr (DT == PCCL_F32) {
+    if (n.elems == 4) return n.lanes == kWave ? f(std::false_type{}, Four{}) : f(std::true_type{}, Four{});
+  }
   if (n.lanes == kWave) f(std::false_type{}, Eight{});
   else if (n.elems == 8) f(std::true_type{}, Eight{});
   else f(std::true_type{}, Sixteen{});
 }
 
 template <int DT, bool PF32> hipError_t launch_fold_norm(NormShape n, bool stream_in, hipStream_t stream, const ForwardArgs &a);
-template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a);
+template <int DT, bool PF32> hipError_t launch_fold_norm_backward(NormShape n, bool single, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a);
 template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, hipStream_t stream, const SumsArgs &a);
 
 #define PCCL_DEFINE_FOLD_NORM(DT, PF32)                                                                                         \
   template <> hipError_t launch_fold_norm<DT, PF32>(NormShape n, bool stream_in, hipStream_t stream, const ForwardArgs &a) {    \
-    with_norm_shape(n, [&](auto team, auto e) {                                                                                 \
+    with_norm_shape<DT>(n, [&](auto team, auto e) {                                                                             \
       constexpr bool TEAM = decltype(team)::value;                                                                              \
       constexpr int E = decltype(e)::value;                                                                                     \
       constexpr int kMany = DT == PCCL_F32 && E == 16 ? 2 : 8; /* eight inputs of 64 bytes a lane would spill */                \
@@ -679,22 +684,22 @@ template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, h
     });                                                                                                                         \
     return hipGetLastError();                                                                                                   \
   }                                                                                                                             \
-  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a) { \
-    with_norm_shape(n, [&](auto team, auto e) {                                                                                 \
+  template <> hipError_t launch_fold_norm_backward<DT, PF32>(NormShape n, bool single, bool bias, bool stream_in, hipStream_t stream, const BackwardArgs &a) { \
+    with_norm_shape<DT>(n, [&](auto team, auto e) {                                                                             \
       constexpr bool TEAM = decltype(team)::value;                                                                              \
       constexpr int E = decltype(e)::value;                                                                                     \
       const dim3 grid(n.workgroups(a.n_teams)), block(n.block());                                                               \
       const unsigned lds = backward_lds(n.block(), E, bias);                                                                    \
-      auto run = [&](auto single, auto b, auto st) {                                                                            \
-        hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, TEAM, E, decltype(single)::value, decltype(b)::value, decltype(st)::value>), \
+      auto run = [&](auto ahead, auto b, auto st) {                                                                             \
+        hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, TEAM, E, decltype(ahead)::value, decltype(b)::value, decltype(st)::value>), \
                            grid, block, lds, stream, a);                                                                        \
       };                                                                                                                        \
       constexpr bool kAhead = row_ahead<DT, E>();                                                                               \
-      if (kAhead && a.n_in == 1 && a.n_out <= 1) {                                                                              \
+      if (kAhead && single) {                                                                                                   \
         typedef std::integral_constant<bool, kAhead> Single;                                                                    \
         if (stream_in) bias ? run(Single{}, std::true_type{}, std::true_type{}) : run(Single{}, std::false_type{}, std::true_type{}); \
         else bias ? run(Single{}, std::true_type{}, std::false_type{}) : run(Single{}, std::false_type{}, std::false_type{});   \
-      } else {                                                                                                                  \
+      } else if constexpr (E > 4) { /* (one pack of binary32 only with a row ahead) */                                          \
         typedef std::integral_constant<bool, !kAhead> Streams; /* (16-bit rows of several gradients: 85 against 88 us, not worth a variant) */ \
         if (stream_in) bias ? run(std::false_type{}, std::true_type{}, Streams{}) : run(std::false_type{}, std::false_type{}, Streams{}); \
         else bias ? run(std::false_type{}, std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{}, std::false_type{}); \
