@@ -114,37 +114,47 @@ struct Share {
   }
   __device__ __forceinline__ bool has(int j) const { return lo[j] < R::kPack; }
 
-  // this lane's packs of the row at `row` (wave-uniform), zeros where it has none
+  // this lane's pack j of the row at `row` (wave-uniform), zeros where it has none
   // (STREAM: non-temporal)
-  template <bool STREAM = false> __device__ __forceinline__ void load(const char *row, u32x4 (&v)[kPacks]) const {
+  template <bool STREAM = false> __device__ __forceinline__ u32x4 load_pack(const char *row, int j) const {
+    u32x4 v{0, 0, 0, 0};
+    if (has(j)) {
+      if (narrow) {
+        typename R::elem_t e[R::kPack];
 #pragma unroll
-    for (int j = 0; j < kPacks; ++j) {
-      v[j] = u32x4{0, 0, 0, 0};
-      if (has(j)) {
-        if (narrow) {
-          typename R::elem_t e[R::kPack];
-#pragma unroll
-          for (int i = 0; i < R::kPack; ++i) e[i] = i >= lo[j] ? ((const typename R::elem_t *)row)[off[j] + i] : (typename R::elem_t)0;
-          v[j] = __builtin_bit_cast(u32x4, e);
-        } else {
-          const typename R::pack_t *at = (const typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes);
-          if constexpr (STREAM) v[j] = __builtin_nontemporal_load(at);
-          else v[j] = *at;
-        }
+        for (int i = 0; i < R::kPack; ++i) e[i] = i >= lo[j] ? ((const typename R::elem_t *)row)[off[j] + i] : (typename R::elem_t)0;
+        v = __builtin_bit_cast(u32x4, e);
+      } else {
+        const typename R::pack_t *at = (const typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes);
+        if constexpr (STREAM) v = __builtin_nontemporal_load(at);
+        else v = *at;
       }
     }
+    return v;
+  }
+  template <bool STREAM = false> __device__ __forceinline__ void load(const char *row, u32x4 (&v)[kPacks]) const {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) v[j] = load_pack<STREAM>(row, j);
   }
   // Rows are stored non-temporally at every size (forward f32 2 -> 2 at 4096 x 2048 45 -> 38 us, bf16 8 -> 8 at 2048 x 8192 129 -> 122).
+  __device__ __forceinline__ void store_pack(char *row, int j, const float *x) const {
+    if (lo[j] == 0) {
+      __builtin_nontemporal_store(R::down(x), (typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes));
+    } else if (has(j)) {
+#pragma unroll
+      for (int i = 0; i < R::kPack; ++i)
+        if (i >= lo[j]) ((typename R::elem_t *)row)[off[j] + i] = R::down1(x[i]);
+    }
+  }
   __device__ __forceinline__ void store(char *row, const float (&x)[E]) const {
 #pragma unroll
-    for (int j = 0; j < kPacks; ++j) {
-      if (lo[j] == 0) {
-        __builtin_nontemporal_store(R::down(x + j * R::kPack), (typename R::pack_t *)(row + (unsigned)off[j] * (unsigned)R::kBytes));
-      } else if (has(j)) {
+    for (int j = 0; j < kPacks; ++j) store_pack(row, j, x + j * R::kPack);
+  }
+  __device__ __forceinline__ void mask_pack(int j, float (&x)[R::kPack]) const {
+    if (ragged && lo[j] != 0) {
 #pragma unroll
-        for (int i = 0; i < R::kPack; ++i)
-          if (i >= lo[j]) ((typename R::elem_t *)row)[off[j] + i] = R::down1(x[j * R::kPack + i]);
-      }
+      for (int i = 0; i < R::kPack; ++i)
+        if (i < lo[j]) x[i] = 0.0f;
     }
   }
   // x = 0 in the elements that are not this lane's; wavefronts whose packs are all whole step over it
@@ -174,38 +184,52 @@ struct ParamShare {
   static constexpr int kWords = kWide ? 2 * kPacks : kPacks;
   u32x4 v[kWords];
 
-  __device__ __forceinline__ void load(const Share<R, TEAM, E> &s, const char *row) {
+  // one pack's
+  static __device__ __forceinline__ void load_pack(const Share<R, TEAM, E> &s, const char *row, int j, u32x4 (&v)[kWords / kPacks]) {
     if constexpr (!kWide) {
-      s.load(row, v);
+      v[0] = s.load_pack(row, j);
     } else {
+      v[0] = v[1] = u32x4{0, 0, 0, 0};
+      if (s.has(j)) {
+        if (s.narrow) {
+          unsigned int e[8];
 #pragma unroll
-      for (int j = 0; j < kPacks; ++j) {
-        v[2 * j] = v[2 * j + 1] = u32x4{0, 0, 0, 0};
-        if (s.has(j)) {
-          if (s.narrow) {
-            unsigned int e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = i >= s.lo[j] ? ((const unsigned int *)row)[s.off[j] + i] : 0u;
-            v[2 * j] = u32x4{e[0], e[1], e[2], e[3]};
-            v[2 * j + 1] = u32x4{e[4], e[5], e[6], e[7]};
-          } else {
-            const u32x4_a4 *at = (const u32x4_a4 *)(row + (unsigned)s.off[j] * 4u);
-            v[2 * j] = at[0];
-            v[2 * j + 1] = at[1];
-          }
+          for (int i = 0; i < 8; ++i) e[i] = i >= s.lo[j] ? ((const unsigned int *)row)[s.off[j] + i] : 0u;
+          v[0] = u32x4{e[0], e[1], e[2], e[3]};
+          v[1] = u32x4{e[4], e[5], e[6], e[7]};
+        } else {
+          const u32x4_a4 *at = (const u32x4_a4 *)(row + (unsigned)s.off[j] * 4u);
+          v[0] = at[0];
+          v[1] = at[1];
         }
       }
     }
   }
-  __device__ __forceinline__ void up(float (&x)[E]) const {
+  static __device__ __forceinline__ void up_pack(const u32x4 *v, float *x) {
     if constexpr (!kWide) {
-      Share<R, TEAM, E>::up(v, x);
+      R::up(v[0], x);
     } else {
 #pragma unroll
-      for (int w = 0; w < kWords; ++w)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * w + i] = as_f32(v[w][i]);
+      for (int i = 0; i < 8; ++i) x[i] = as_f32(v[i / 4][i % 4]);
     }
+  }
+  static __device__ __forceinline__ void pack(const Share<R, TEAM, E> &s, const char *row, int j, float (&x)[R::kPack]) {
+    u32x4 w[kWords / kPacks];
+    load_pack(s, row, j, w);
+    up_pack(w, x);
+  }
+  __device__ __forceinline__ void load(const Share<R, TEAM, E> &s, const char *row) {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) {
+      u32x4 w[kWords / kPacks];
+      load_pack(s, row, j, w);
+#pragma unroll
+      for (int k = 0; k < kWords / kPacks; ++k) v[j * (kWords / kPacks) + k] = w[k];
+    }
+  }
+  __device__ __forceinline__ void up(float (&x)[E]) const {
+#pragma unroll
+    for (int j = 0; j < kPacks; ++j) up_pack(v + j * (kWords / kPacks), x + j * R::kPack);
   }
 };
 

@@ -190,19 +190,21 @@ struct Columns {
       for (int i = 0; i < E; ++i) x[i] = 0.0f;
     }
   }
-  // += a * b, element by element
-  __device__ __forceinline__ void add(const float (&a)[E], const float (&b)[E]) {
+  // += a * b, element by element: N columns from `first` on
+  template <int N>
+  __device__ __forceinline__ void add(int first, const float (&a)[N], const float (&b)[N]) {
     if constexpr (IN_LDS) {
 #pragma unroll
-      for (int k = 0; k < E / 4; ++k) {
-        f32x4 v = at[k * step];
+      for (int k = 0; k < N / 4; ++k) {
+        f32x4 &to = at[(first / 4 + k) * step];
+        f32x4 v = to;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(a[4 * k + i], b[4 * k + i], v[i]);
-        at[k * step] = v;
+        to = v;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = __builtin_fmaf(a[i], b[i], x[i]);
+      for (int i = 0; i < N; ++i) x[first + i] = __builtin_fmaf(a[i], b[i], x[first + i]);
     }
   }
   __device__ __forceinline__ void get(float (&to)[E]) const {
@@ -222,9 +224,12 @@ struct Columns {
 // One team's registers hold the row (packed), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, s1 and p1.
 // Rows of one pack a lane (16-bit up to 8192 columns, binary32 up to 4096) that are four streams (SINGLE: one y and at most one dh) have
 // room for the row after it, on its way; binary32 with two packs spilled with it (8192 x 2048 87 -> 84 us without, 78 with one pack
-// and the row ahead).  s0 and p0 and the post norm's sums over a
-// team's strips stay in LDS.  Wider rows (E = 16) keep s1 and p1 there instead, the post norm's sums over strips go to the
-// workspace and back.
+// and the row ahead).  s0 and p0 and the post norm's sums over a team's strips stay in LDS.
+// Rows beyond 8192 columns (E = 16) have sixteen wavefronts, all of a compute unit's registers, 8 for each column.  They go pack by pack,
+// in order: what a pack needs of wpre and cgw is read from the caches as it comes, y, r and dh stay as they were loaded and are unpacked and
+// centred anew in each phase, s1 and p1 are in LDS, the post norm's sums over strips go to the workspace and back, and only 16-bit rows
+// without BIAS have the next row on its way.  (2048 x 16384 bf16 113 -> 106 us, with biases 226 -> 131; f32 1024 x 16384 148 -> 105: the
+// whole row at once spilled 18 to 123 registers.)
 // BIAS: some bias's gradient or a gate behind a biased norm is asked for (s0 and p0 are kept).
 // STREAM: rows are read non-temporally.
 //
@@ -240,8 +245,10 @@ struct BackRow {
   u32x4 y[E / R::kPack], r[E / R::kPack], dh[E / R::kPack], dr[E / R::kPack];
 };
 
-template <int DT, int E>
-constexpr bool row_ahead() { return E == RowType<DT>::kPack; }
+// Whether calls of one y and at most one dh have instances of their own: all but two packs of binary32 in one wavefront (50000 x 400
+// 92 us without, 97 with; beyond 4096 columns 2048 x 8192 88 -> 84).
+template <int DT, bool TEAM, int E>
+constexpr bool row_single() { return E == RowType<DT>::kPack || TEAM; }
 
 template <int DT, bool PF32, bool TEAM, int E, bool SINGLE, bool BIAS, bool STREAM>
 __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel(const BackwardArgs) {
@@ -250,7 +257,9 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
   typedef ParamShare<R, PF32, TEAM, E> P;
   constexpr int kTeams = TEAM ? 1 : kBlock / kWave;
   constexpr bool kWide = E > 8;
-  constexpr int kFold = 4;  // gradients in flight together; more cost registers
+  constexpr int kPack = R::kPack, kPacks = E / kPack;
+  constexpr bool kNext = SINGLE && (E == R::kPack || (R::kBytes == 2 && !BIAS));  // the next row is on its way
+  constexpr int kFold = E * R::kBytes > 32 ? 1 : E * R::kBytes > 16 ? 2 : 4;  // gradients in flight together; more cost registers
   const BackwardArgsAt args = (BackwardArgsAt)__builtin_amdgcn_kernarg_segment_ptr();  // (the one argument stands at its start)
   const BackwardArgsAt a0 = args;
   __shared__ float words[2][TEAM ? kMostWaves : 1][kSumsAtOnce];
@@ -265,49 +274,54 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
   const bool post_layer = a0->post_kind == PCCL_NORM_LAYER, pre_layer = pre && a0->pre_kind == PCCL_NORM_LAYER;
   const float per_width = a0->per_width;
 
-  float wpre_kept[kWide ? 1 : E], ones[E];
+  float wpre_kept[kWide ? 1 : E], ones[kPack];
   Columns<E, kWide> p1{{}, columns(0), (int)blockDim.x}, s1{{}, columns(1), (int)blockDim.x};
   Columns<E, !kWide> p0{{}, columns(2), (int)blockDim.x}, s0{{}, columns(3), (int)blockDim.x};                   // (BIAS)
   Columns<E, true> post_sums{{}, columns(0), (int)blockDim.x}, post_bias_sums{{}, columns(1), (int)blockDim.x};  // (E up to 8)
   p1.zero();
   if constexpr (BIAS) p0.zero();
 #pragma unroll
-  for (int i = 0; i < E; ++i) ones[i] = 1.0f;
-  // wpre and cgw: with E = 16 read again (from the caches) wherever a row needs them
-  auto get_wpre = [&](float (&to)[E]) {
+  for (int i = 0; i < kPack; ++i) ones[i] = 1.0f;
+  // wpre and cgw: with E = 16 read again (from the caches), pack by pack, wherever a row needs them
+  auto get_wpre = [&](int j, float (&to)[kPack]) {
     const BackwardArgsAt a = read_again(args);
 #pragma unroll
-    for (int i = 0; i < E; ++i) to[i] = 1.0f;
+    for (int i = 0; i < kPack; ++i) to[i] = 1.0f;
     if (a->pre_weight) {
-      P w;
-      w.load(s, a->pre_weight);
-      w.up(to);
+      P::pack(s, a->pre_weight, j, to);
 #pragma unroll
-      for (int i = 0; i < E; ++i) to[i] += a->weight_offset;
+      for (int i = 0; i < kPack; ++i) to[i] += a->weight_offset;
     }
   };
-  auto get_cgw = [&](unsigned group, float (&to)[E]) {
+  auto get_cgw = [&](unsigned group, int j, float (&to)[kPack]) {
     const BackwardArgsAt a = read_again(args);
 #pragma unroll
-    for (int i = 0; i < E; ++i) to[i] = a->block_scale;
+    for (int i = 0; i < kPack; ++i) to[i] = a->block_scale;
     if (a->gate) {
-      P g;
-      float f[E];
-      g.load(s, a->gate + group * a->gate_bytes);
-      g.up(f);
+      float f[kPack];
+      P::pack(s, a->gate + group * a->gate_bytes, j, f);
 #pragma unroll
-      for (int i = 0; i < E; ++i) to[i] *= f[i];
+      for (int i = 0; i < kPack; ++i) to[i] *= f[i];
     }
     if (a->post_weight) {
-      P w;
-      float f[E];
-      w.load(s, a->post_weight);
-      w.up(f);
+      float f[kPack];
+      P::pack(s, a->post_weight, j, f);
 #pragma unroll
-      for (int i = 0; i < E; ++i) to[i] *= f[i] + a->weight_offset;
+      for (int i = 0; i < kPack; ++i) to[i] *= f[i] + a->weight_offset;
     }
   };
-  if constexpr (!kWide) get_wpre(wpre_kept);
+  auto all = [&](auto &&get, float (&to)[kWide ? 1 : E]) {
+    if constexpr (!kWide) {
+#pragma unroll
+      for (int j = 0; j < kPacks; ++j) {
+        float x[kPack];
+        get(j, x);
+#pragma unroll
+        for (int i = 0; i < kPack; ++i) to[j * kPack + i] = x[i];
+      }
+    }
+  };
+  all(get_wpre, wpre_kept);
 
   auto load_row = [&](unsigned long row, BackRow<R, E> &x) {
     const BackwardArgsAt a = read_again(args);
@@ -330,142 +344,220 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
     const unsigned step = a1->strips;
 
     BackRow<R, E> next;
-    if (SINGLE && begin < stop) load_row(begin, next);
+    if (kNext && begin < stop) load_row(begin, next);
     s1.zero();
     if constexpr (BIAS) s0.zero();
     float cgw_kept[kWide ? 1 : E];
-    if constexpr (!kWide) get_cgw(group, cgw_kept);
+    all([&](int j, float (&to)[kPack]) { get_cgw(group, j, to); }, cgw_kept);
 
     for (unsigned long row = begin; row < stop; row += step) {
       BackRow<R, E> now;
-      float y[E], dh[E], r[E];
-      if constexpr (SINGLE) {
+      float y_kept[E], dh_kept[E], r_kept[E];  // (those that are not unpacked anew)
+      if constexpr (kNext) {
         now = next;
         if (row + step < stop) load_row(row + step, next);
-        s.up(now.y, y);
-        if (outs) s.up(now.dh, dh);
       } else {
         load_row(row, now);
+      }
+      if constexpr (!SINGLE) {
         const BackwardArgsAt a = read_again(args);
-        if (outs) fold_rows<STREAM, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh);
-        fold_rows<STREAM, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y);
+        if (outs) fold_rows<STREAM, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh_kept);
+        fold_rows<STREAM, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y_kept);
+      } else if constexpr (!kWide) {
+        s.up(now.y, y_kept);
+        if (outs) s.up(now.dh, dh_kept);
       }
-      s.mask(y);
-      if (outs) s.mask(dh);
-      if (pre) {
-        s.up(now.r, r);
-        s.mask(r);
+      if constexpr (!(SINGLE && kWide)) {
+        s.mask(y_kept);
+        if (outs) s.mask(dh_kept);
       }
+      if constexpr (!kWide) {
+        if (pre) {
+          s.up(now.r, r_kept);
+          s.mask(r_kept);
+        }
+      }
+      // pack j of y, dh and r, y and r less their means once those are known
+      float mean_y = 0.0f, mean_r = 0.0f;
+      auto unpacked = [&](u32x4 v, int j, float mean, float (&to)[kPack]) {
+        asm volatile("" : "+v"(v));  // (no instruction: the compiler may not keep what it unpacked before)
+        R::up(v, to);
+#pragma unroll
+        for (int i = 0; i < kPack; ++i) to[i] -= mean;
+        s.mask_pack(j, to);
+      };
+      auto kept = [&](const float (&x)[E], int j, float (&to)[kPack]) {
+#pragma unroll
+        for (int i = 0; i < kPack; ++i) to[i] = x[j * kPack + i];
+      };
+      auto get_y = [&](int j, float (&to)[kPack]) {
+        if constexpr (SINGLE && kWide) unpacked(now.y[j], j, mean_y, to);
+        else kept(y_kept, j, to);
+      };
+      auto get_dh = [&](int j, float (&to)[kPack]) {
+        if constexpr (SINGLE && kWide) unpacked(now.dh[j], j, 0.0f, to);
+        else kept(dh_kept, j, to);
+      };
+      auto get_r = [&](int j, float (&to)[kPack]) {
+        if constexpr (kWide) unpacked(now.r[j], j, mean_r, to);
+        else kept(r_kept, j, to);
+      };
+      auto wpre = [&](int j, float (&to)[kPack]) {
+        if constexpr (kWide) get_wpre(j, to);
+        else kept(wpre_kept, j, to);
+      };
+      auto cgw = [&](int j, float (&to)[kPack]) {
+        if constexpr (kWide) get_cgw(group, j, to);
+        else kept(cgw_kept, j, to);
+      };
+      // packs one after the other: what one of them needs is not loaded before the last is done with
+      auto packs = [&](auto &&work) {
+#pragma unroll
+        for (int j = 0; j < kPacks; ++j) {
+          if (!kWide || j == 0 || __builtin_amdgcn_readfirstlane(s.lo[j]) < kPack) work(j);  // (a wavefront may be behind the row's end)
+          if constexpr (kWide) __builtin_amdgcn_sched_barrier(0);
+        }
+      };
       // both norms' statistics, and what the pre norm's backward sums, in one go over the team (two with a layer norm)
       if (post_layer || pre_layer) {
         float m[2] = {0.0f, 0.0f};
-        if (post_layer) {
+        packs([&](int j) {
+          float x[kPack];
+          if (post_layer) {
+            get_y(j, x);
 #pragma unroll
-          for (int i = 0; i < E; ++i) m[0] += y[i];
-        }
-        if (pre_layer) {
+            for (int i = 0; i < kPack; ++i) m[0] += x[i];
+          }
+          if (pre_layer) {
+            get_r(j, x);
 #pragma unroll
-          for (int i = 0; i < E; ++i) m[1] += r[i];
-        }
+            for (int i = 0; i < kPack; ++i) m[1] += x[i];
+          }
+        });
         sums(m);
         if (post_layer) {
-          const float mean = m[0] * per_width;
+          mean_y = m[0] * per_width;
+          if constexpr (!(SINGLE && kWide)) {
 #pragma unroll
-          for (int i = 0; i < E; ++i) y[i] -= mean;
-          s.mask(y);
+            for (int i = 0; i < E; ++i) y_kept[i] -= mean_y;
+            s.mask(y_kept);
+          }
         }
         if (pre_layer) {
-          const float mean = m[1] * per_width;
+          mean_r = m[1] * per_width;
+          if constexpr (!kWide) {
 #pragma unroll
-          for (int i = 0; i < E; ++i) r[i] -= mean;
-          s.mask(r);
+            for (int i = 0; i < E; ++i) r_kept[i] -= mean_r;
+            s.mask(r_kept);
+          }
         }
       }
       float q[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // squares of y, squares of r, dh * w * r, dh * w
-      if (post) {
+      packs([&](int j) {
+        if (post) {
+          float y[kPack];
+          get_y(j, y);
 #pragma unroll
-        for (int i = 0; i < E; ++i) q[0] = __builtin_fmaf(y[i], y[i], q[0]);
-      }
-      if (pre) {
-        float w[kWide ? E : 1];
-        if constexpr (kWide) get_wpre(w);
-        const auto &wpre = [&]() -> const float (&)[E] { if constexpr (kWide) return w; else return wpre_kept; }();
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          q[1] = __builtin_fmaf(r[i], r[i], q[1]);
-          q[2] = __builtin_fmaf(dh[i] * wpre[i], r[i], q[2]);
+          for (int i = 0; i < kPack; ++i) q[0] = __builtin_fmaf(y[i], y[i], q[0]);
         }
-        if (pre_layer) {
+        if (pre) {
+          float r[kPack], dh[kPack], w[kPack];
+          wpre(j, w);
+          get_r(j, r);
+          get_dh(j, dh);
 #pragma unroll
-          for (int i = 0; i < E; ++i) q[3] = __builtin_fmaf(dh[i], wpre[i], q[3]);
+          for (int i = 0; i < kPack; ++i) {
+            q[1] = __builtin_fmaf(r[i], r[i], q[1]);
+            q[2] = __builtin_fmaf(dh[i] * w[i], r[i], q[2]);
+          }
+          if (pre_layer) {
+#pragma unroll
+            for (int i = 0; i < kPack; ++i) q[3] = __builtin_fmaf(dh[i], w[i], q[3]);
+          }
         }
-      }
+      });
       if (post || pre) sums(q);
       const BackwardArgsAt a = read_again(args);
-      float dr[E];
-      if (a->grad_residual_out) {
-        s.up(now.dr, dr);
-      } else {
+      float dr[E] = {};
+      // dr += rstd * (d - rhat * mean(d * rhat) - mean(d)), d = dh * w
+      const float pre_rstd = one_over_spread(q[1], per_width, a->pre_eps);
+      const float pre_along = -pre_rstd * (q[2] * per_width);  // (no power of rstd on its own: with a tiny eps that could pass the largest binary32)
+      const float pre_mean = pre_rstd * (q[3] * per_width);
+      packs([&](int j) {
+        float d[kPack], dh[kPack];
+        if (a->grad_residual_out) {
+          R::up(now.dr[j], d);
+        } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] = 0.0f;
-      }
-      if (pre) {
-        // dr += rstd * (d - rhat * mean(d * rhat) - mean(d)), d = dh * w
-        const float rstd = one_over_spread(q[1], per_width, a->pre_eps);
-        const float along = -rstd * (q[2] * per_width);  // (no power of rstd on its own: with a tiny eps that could pass the largest binary32)
-        float w[kWide ? E : 1];
-        if constexpr (kWide) get_wpre(w);
-        const auto &wpre = [&]() -> const float (&)[E] { if constexpr (kWide) return w; else return wpre_kept; }();
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          r[i] *= rstd;
-          dr[i] = __builtin_fmaf(rstd, __builtin_fmaf(r[i], along, dh[i] * wpre[i]), dr[i]);
+          for (int i = 0; i < kPack; ++i) d[i] = 0.0f;
         }
-        p1.add(dh, r);
-        if (pre_layer) {
-          const float mean = rstd * (q[3] * per_width);
+        if (pre) {
+          float w[kPack], r[kPack];
+          wpre(j, w);
+          get_r(j, r);
+          get_dh(j, dh);
 #pragma unroll
-          for (int i = 0; i < E; ++i) dr[i] -= mean;
+          for (int i = 0; i < kPack; ++i) {
+            r[i] *= pre_rstd;
+            d[i] = __builtin_fmaf(pre_rstd, __builtin_fmaf(r[i], pre_along, dh[i] * w[i]), d[i]);
+          }
+          p1.add(j * kPack, dh, r);
+          if (pre_layer) {
+#pragma unroll
+            for (int i = 0; i < kPack; ++i) d[i] -= pre_mean;
+          }
+          if constexpr (BIAS) p0.add(j * kPack, dh, ones);
+        } else if (outs) {
+          get_dh(j, dh);
+#pragma unroll
+          for (int i = 0; i < kPack; ++i) d[i] += dh[i];
         }
-        if constexpr (BIAS) p0.add(dh, ones);
-      } else if (outs) {
+        s.mask_pack(j, d);
+        if (a->grad_residual) {
+          float x[kPack];
 #pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] += dh[i];
-      }
-      s.mask(dr);
-      if (a->grad_residual) {
-        float x[E];
+          for (int i = 0; i < kPack; ++i) x[i] = a->residual_scale * d[i];
+          s.store_pack(a->grad_residual + row * a->grad_residual_bytes, j, x);
+        }
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = a->residual_scale * dr[i];
-        s.store(a->grad_residual + row * a->grad_residual_bytes, x);
-      }
-      float cgw_read[kWide ? E : 1];
-      if constexpr (kWide) get_cgw(group, cgw_read);
-      const auto &cgw = [&]() -> const float (&)[E] { if constexpr (kWide) return cgw_read; else return cgw_kept; }();
-      if (post) {
-        const float rstd = one_over_spread(q[0], per_width, a->post_eps);
-        float m[2] = {0.0f, 0.0f};
+        for (int i = 0; i < kPack; ++i) dr[j * kPack + i] = d[i];
+      });
+      const float post_rstd = post ? one_over_spread(q[0], per_width, a->post_eps) : 1.0f;
+      float m[2] = {0.0f, 0.0f};
+      packs([&](int j) {
+        float d[kPack], y[kPack], w[kPack];
+        kept(dr, j, d);
+        cgw(j, w);
+        get_y(j, y);
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] *= rstd;
-        s1.add(dr, y);
-        if constexpr (BIAS) s0.add(dr, ones);
+        for (int i = 0; i < kPack; ++i) y[i] *= post_rstd;
+        s1.add(j * kPack, d, y);
+        if constexpr (BIAS)
+          if (post) s0.add(j * kPack, d, ones);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          dr[i] *= cgw[i];
-          m[0] = __builtin_fmaf(dr[i], y[i], m[0]);
+        for (int i = 0; i < kPack; ++i) {
+          d[i] *= w[i];
+          m[0] = __builtin_fmaf(d[i], y[i], m[0]);
+          dr[j * kPack + i] = d[i];
+          if constexpr (!(SINGLE && kWide)) y_kept[j * kPack + i] = y[i];
         }
         if (post_layer) {
 #pragma unroll
-          for (int i = 0; i < E; ++i) m[1] += dr[i];
+          for (int i = 0; i < kPack; ++i) m[1] += d[i];
         }
+      });
+      if (post) {
         sums(m);
-        const float along = -rstd * (m[0] * per_width), mean = -rstd * (m[1] * per_width);
+        const float along = -post_rstd * (m[0] * per_width), mean = -post_rstd * (m[1] * per_width);
+        packs([&](int j) {
+          float y[kPack];
+          get_y(j, y);
 #pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] = __builtin_fmaf(dr[i], rstd, __builtin_fmaf(y[i], along, mean));
-      } else {
-        s1.add(dr, y);
-#pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] *= cgw[i];
+          for (int i = 0; i < kPack; ++i) {
+            if constexpr (SINGLE && kWide) y[i] *= post_rstd;
+            dr[j * kPack + i] = __builtin_fmaf(dr[j * kPack + i], post_rstd, __builtin_fmaf(y[i], along, mean));
+          }
+        });
       }
       const unsigned long at = row * a->grad_in_bytes;
 #pragma unroll 1
@@ -524,8 +616,8 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
           post_sums.zero();
           if constexpr (BIAS) post_bias_sums.zero();
         }
-        post_sums.add(f, x);
-        if constexpr (BIAS) post_bias_sums.add(f, x0);
+        post_sums.add(0, f, x);
+        if constexpr (BIAS) post_bias_sums.add(0, f, x0);
       } else {
         // (each lane adds to the columns that it wrote itself)
         float *mine = a->sums + (unsigned long)t * 4 * a->width;
@@ -694,13 +786,13 @@ template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, h
         hipLaunchKernelGGL((fold_norm_backward_kernel<DT, PF32, TEAM, E, decltype(ahead)::value, decltype(b)::value, decltype(st)::value>), \
                            grid, block, lds, stream, a);                                                                        \
       };                                                                                                                        \
-      constexpr bool kAhead = row_ahead<DT, E>();                                                                               \
-      if (kAhead && single) {                                                                                                   \
-        typedef std::integral_constant<bool, kAhead> Single;                                                                    \
+      constexpr bool kSingle = row_single<DT, TEAM, E>();                                                                       \
+      if (kSingle && single) {                                                                                                  \
+        typedef std::integral_constant<bool, kSingle> Single;                                                                    \
         if (stream_in) bias ? run(Single{}, std::true_type{}, std::true_type{}) : run(Single{}, std::false_type{}, std::true_type{}); \
         else bias ? run(Single{}, std::true_type{}, std::false_type{}) : run(Single{}, std::false_type{}, std::false_type{});   \
       } else if constexpr (E > 4) { /* (one pack of binary32 only with a row ahead) */                                          \
-        typedef std::integral_constant<bool, !kAhead> Streams; /* (16-bit rows of several gradients: 85 against 88 us, not worth a variant) */ \
+        typedef std::integral_constant<bool, !kSingle> Streams; /* (16-bit rows of several gradients: 85 against 88 us, not worth a variant) */ \
         if (stream_in) bias ? run(std::false_type{}, std::true_type{}, Streams{}) : run(std::false_type{}, std::false_type{}, Streams{}); \
         else bias ? run(std::false_type{}, std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{}, std::false_type{}); \
       }                                                                                                                         \
