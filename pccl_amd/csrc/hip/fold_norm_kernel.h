@@ -173,6 +173,25 @@ __device__ __forceinline__ void store_sums(const Share<R, TEAM, E> &s, float *ro
   }
 }
 
+template <class R, bool TEAM, int E>
+__device__ __forceinline__ void load_sums(const Share<R, TEAM, E> &s, const float *row, float (&x)[E]) {
+#pragma unroll
+  for (int j = 0; j < E / R::kPack; ++j) {
+    float *to = x + j * R::kPack;
+    if (s.lo[j] == 0) {
+#pragma unroll
+      for (int w = 0; w < R::kPack / 4; ++w) {
+        const u32x4 v = *(const u32x4_a4 *)(row + s.off[j] + 4 * w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[4 * w + i] = as_f32(v[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::kPack; ++i) to[i] = i >= s.lo[j] ? row[s.off[j] + i] : 0.0f;
+    }
+  }
+}
+
 // Sums over rows that a lane keeps for its columns, in registers or (IN_LDS) in the workgroup's LDS, four columns to a 16-byte
 // word, words of one lane `step` apart.
 template <int E, bool IN_LDS>
@@ -622,12 +641,8 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
         // (each lane adds to the columns that it wrote itself)
         float *mine = a->sums + (unsigned long)t * 4 * a->width;
         auto add = [&](float *row, const float (&v)[E]) {
-          float had[E];
-#pragma unroll
-          for (int j = 0; j < E / R::kPack; ++j)
-#pragma unroll
-            for (int i = 0; i < R::kPack; ++i)
-              had[j * R::kPack + i] = strip != first && i >= s.lo[j] ? row[s.off[j] + i] : 0.0f;
+          float had[E] = {};
+          if (strip != first) load_sums(s, row, had);
 #pragma unroll
           for (int i = 0; i < E; ++i) had[i] = __builtin_fmaf(f[i], v[i], had[i]);
           store_sums(s, row, had);
