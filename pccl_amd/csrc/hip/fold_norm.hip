@@ -18,8 +18,8 @@ constexpr unsigned kLaunchRows = 1u << 21;
 // One pack of 16 bytes a lane while a workgroup holds the row, else two (binary32 beyond 8192 columns: four): a wavefront where one is
 // enough (no barrier in its sums), beyond a workgroup of as many as the width fills.  (binary32 up to 4096 columns with one pack
 // and not two: forward 8192 x 2048 53 -> 48 us, 4096 x 4096 4 -> 2 95 -> 90; backward, where it is what leaves room for a row ahead,
-// 4985 x 1025 50 -> 41, 16384 x 1024 83 -> 80.  Without a row ahead the backward pass loses, 3000 x 4000 of two gradients 94 -> 97, and
-// with rows of 257 to 512 columns, where two packs still are one wavefront's, 50000 x 400 92 -> 97.)
+// 4985 x 1025 50 -> 41, 16384 x 1024 83 -> 80; backward rows of 257 to 512 columns, where two packs still are one wavefront's, lose:
+// 50000 x 400 98 -> 101, 30000 x 300 with biases 59 -> 69.)
 NormShape shape_of(long width, int dtype, bool one_pack) {
   const int elems = dtype == PCCL_F32 && one_pack && width <= 4096 ? 4 : width <= 8192 ? 8 : 16;
   return {(int)((width + elems * kWave - 1) / (elems * kWave)) * kWave, elems};
@@ -126,11 +126,11 @@ int launched(hipError_t e, const char *what) {
   return e == hipSuccess ? PCCL_OK : fail(PCCL_ERR_HIP, "%s launch failed: %s", what, hipGetErrorString(e));
 }
 
-// Shape of the backward pass.  `single`: one y and at most one gradient of h.  Beyond 8192 columns always sixteen wavefronts, some of which
+// Shape of the backward pass.  Beyond 8192 columns always sixteen wavefronts, some of which
 // then have one pack, others two: a compute unit holds no second team (bf16 4096 x 9216 138 -> 124 us, 2048 x 12288 93 -> 89).
-NormShape backward_shape(long width, int dtype, bool single) {
+NormShape backward_shape(long width, int dtype) {
   if (width > 8192) return {kMostLanes, 16};
-  return shape_of(width, dtype, single && (width <= 4 * kWave || width > 8 * kWave));
+  return shape_of(width, dtype, width <= 4 * kWave || width > 8 * kWave);
 }
 
 // How the backward pass cuts the rows (see BackwardArgs).
@@ -141,11 +141,11 @@ struct Cut {
 // Teams that fill the chip: enough for several wavefronts on every SIMD, few enough that writing and joining their sums
 // (4 rows of binary32 a team) stays small beside the rows themselves.  Twelve wavefronts a compute unit (or the team that
 // passes twelve) where teams have their next row on its way, sixteen where they wait for it: without a row ahead, and with
-// gate rows so short that a strip has none (`ahead` with 12 against 16: 8000 x 1536 bf16, 8 gate rows, 51 -> 48 us, 100000 x 200
-// f32 96 -> 88; 8192 x 2048 with a gate a row 65 -> 68, 4096 x 4096 of four gradients 89 -> 107).
-Cut cut_of(long rows, long width, long gate_rows, int dtype, bool single) {
-  const NormShape n = backward_shape(width, dtype, single);
-  const bool ahead = single && n.elems * pccl_host::pccl_dtype_bytes(dtype) == 16;
+// gate rows so short that a strip has none (12 against 16: 8000 x 1536 bf16, 8 gate rows, 51 -> 48 us, 100000 x 200 f32 96 -> 88;
+// 8192 x 2048 with a gate a row 65 -> 68).
+Cut cut_of(long rows, long width, long gate_rows, int dtype) {
+  const NormShape n = backward_shape(width, dtype);
+  const bool ahead = n.elems * pccl_host::pccl_dtype_bytes(dtype) == 16;
   const long per = gate_rows >= 1 ? std::min(gate_rows, std::max(1l, rows)) : std::max(1l, rows);
   int teams = kMostLanes / n.lanes;
   if (ahead && per >= 4) teams = std::min(teams, (12 * kWave + n.lanes - 1) / n.lanes);
@@ -212,11 +212,9 @@ extern "C" int pccl_hip_fold_norm_workspace(long rows, long width, long gate_row
   if (rows < 0 || rows > 0x7fffffffl) return fail(PCCL_ERR_INVALID_ARG, "rows %ld outside [0, 2^31)", rows);
   if (width < 1 || width > PCCL_NORM_MAX_WIDTH) return fail(PCCL_ERR_INVALID_ARG, "width %ld outside [1, %d]", width, PCCL_NORM_MAX_WIDTH);
   if (gate_rows < 0) return fail(PCCL_ERR_INVALID_ARG, "gate_rows %ld < 0", gate_rows);
-  for (int dtype : {PCCL_F32, PCCL_BF16}) {  // whichever type the rows have, and however many gradients there are
-    for (bool single : {false, true}) {
-      const Cut c = cut_of(rows, width, gate_rows, dtype, single);
-      *bytes = std::max(*bytes, sums_bytes(c, width) + (gate_rows ? gate_sums_bytes(c, width) : 0));
-    }
+  for (int dtype : {PCCL_F32, PCCL_BF16}) {  // whichever type the rows have
+    const Cut c = cut_of(rows, width, gate_rows, dtype);
+    *bytes = std::max(*bytes, sums_bytes(c, width) + (gate_rows ? gate_sums_bytes(c, width) : 0));
   }
   return PCCL_OK;
 }
@@ -255,8 +253,8 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
   }
   if (c.rc != PCCL_OK) return c.rc;
   const bool single = d->n_in == 1 && d->n_out <= 1;
-  const NormShape shape = backward_shape(d->width, d->dtype, single);
-  const Cut cut = cut_of(d->rows, d->width, d->gate ? d->gate_rows : 0, d->dtype, single);
+  const NormShape shape = backward_shape(d->width, d->dtype);
+  const Cut cut = cut_of(d->rows, d->width, d->gate ? d->gate_rows : 0, d->dtype);
   const bool joined_gate = g->grad_gate && cut.strips > 1;
   const long need = (any ? sums_bytes(cut, d->width) : 0) + (joined_gate ? gate_sums_bytes(cut, d->width) : 0);
   if (need) {

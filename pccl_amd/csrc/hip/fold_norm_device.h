@@ -233,11 +233,11 @@ struct ParamShare {
   }
 };
 
-// y = the left fold of this lane's share of n rows.  AT_ONCE inputs are in flight together.
-template <bool STREAM, int AT_ONCE, class R, bool TEAM, int E, class Ins>
+// y = the left fold of this lane's share of n rows; FROM = 1: y holds the first of them already.  AT_ONCE inputs are in flight together.
+template <bool STREAM, int AT_ONCE, int FROM, class R, bool TEAM, int E, class Ins>
 __device__ __forceinline__ void fold_rows(const Share<R, TEAM, E> &s, const Ins &ins, int n, long at, float (&y)[E]) {
   constexpr int kPacks = E / R::kPack;
-  for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
+  for (int k0 = FROM; k0 < n; k0 += AT_ONCE) {
     u32x4 v[AT_ONCE][kPacks];
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k)

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(team_block(TEAM)) fold_norm_kernel(const Forwa
   u32x4 x[E / R::kPack];
   float v[E];
   if (a.residual) s.template load<STREAM>(a.residual + (long)row * a.residual_bytes, x);
-  fold_rows<STREAM, AT_ONCE>(s, a.ins, a.n_in, (long)row * a.in_bytes, v);
+  fold_rows<STREAM, AT_ONCE, 0>(s, a.ins, a.n_in, (long)row * a.in_bytes, v);
   s.mask(v);
   // parameters come from the caches; asked for in front of the sums that they are waited for behind
   if (a.post_weight) post_weight.load(s, a.post_weight);
@@ -241,9 +241,9 @@ struct Columns {
 // so that a row costs one fused multiply-add a column for each, and gate and weight are met once a strip.
 //
 // One team's registers hold the row (packed), wpre = w + o of the pre norm, cgw = c * g * (w + o) of the post norm, s1 and p1.
-// Rows of one pack a lane (16-bit up to 8192 columns, binary32 up to 4096) that are four streams (SINGLE: one y and at most one dh) have
-// room for the row after it, on its way; binary32 with two packs spilled with it (8192 x 2048 87 -> 84 us without, 78 with one pack
-// and the row ahead).  s0 and p0 and the post norm's sums over a team's strips stay in LDS.
+// Rows of one pack a lane (16-bit up to 8192 columns, binary32 up to 4096) have room for the row after it, on its way; of several partial
+// y or dh (SINGLE: there are none) the first, the others are loaded four at once when the row's turn comes (bf16 4096 x 4096 of two
+// gradients 58 -> 55 us).  binary32 with two packs spilled with it (8192 x 2048 87 -> 84 us without, 78 with one pack and the row ahead).  s0 and p0 and the post norm's sums over a team's strips stay in LDS.
 // Rows beyond 8192 columns (E = 16) have sixteen wavefronts, all of a compute unit's registers, 8 for each column.  They go pack by pack,
 // in order: what a pack needs of wpre and cgw is read from the caches as it comes, y, r and dh stay as they were loaded and are unpacked and
 // centred anew in each phase, s1 and p1 are in LDS, the post norm's sums over strips go to the workspace and back, and only 16-bit rows
@@ -265,7 +265,7 @@ struct BackRow {
 };
 
 // Whether calls of one y and at most one dh have instances of their own: all but two packs of binary32 in one wavefront (50000 x 400
-// 92 us without, 97 with; beyond 4096 columns 2048 x 8192 88 -> 84).
+// 98 us with and without; beyond 4096 columns 2048 x 8192 88 -> 84).
 template <int DT, bool TEAM, int E>
 constexpr bool row_single() { return E == RowType<DT>::kPack || TEAM; }
 
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
   constexpr int kTeams = TEAM ? 1 : kBlock / kWave;
   constexpr bool kWide = E > 8;
   constexpr int kPack = R::kPack, kPacks = E / kPack;
-  constexpr bool kNext = SINGLE && (E == R::kPack || (R::kBytes == 2 && !BIAS));  // the next row is on its way
+  constexpr bool kNext = E == R::kPack || (SINGLE && R::kBytes == 2 && !BIAS);  // the next row is on its way
   constexpr int kFold = E * R::kBytes > 32 ? 1 : E * R::kBytes > 16 ? 2 : 4;  // gradients in flight together; more cost registers
   const BackwardArgsAt args = (BackwardArgsAt)__builtin_amdgcn_kernarg_segment_ptr();  // (the one argument stands at its start)
   const BackwardArgsAt a0 = args;
@@ -346,10 +346,8 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
     const BackwardArgsAt a = read_again(args);
     if (a->grad_residual_out) s.template load<STREAM>(a->grad_residual_out + row * a->grad_residual_out_bytes, x.dr);
     if (pre) s.template load<STREAM>(a->residual_out + row * a->residual_out_bytes, x.r);
-    if constexpr (SINGLE) {
-      if (outs) s.template load<STREAM>(a->grad_outs[0] + row * a->grad_out_bytes, x.dh);
-      s.template load<STREAM>(a->ins[0] + row * a->in_bytes, x.y);
-    }
+    if (outs) s.template load<STREAM>(a->grad_outs[0] + row * a->grad_out_bytes, x.dh);
+    s.template load<STREAM>(a->ins[0] + row * a->in_bytes, x.y);
   };
 
   const unsigned first = (unsigned)((unsigned long)a0->n_strips * t / a0->n_teams);
@@ -378,13 +376,14 @@ __global__ void __launch_bounds__(team_block(TEAM), 4) fold_norm_backward_kernel
       } else {
         load_row(row, now);
       }
-      if constexpr (!SINGLE) {
-        const BackwardArgsAt a = read_again(args);
-        if (outs) fold_rows<STREAM, kFold>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh_kept);
-        fold_rows<STREAM, kFold>(s, a->ins, a->n_in, row * a->in_bytes, y_kept);
-      } else if constexpr (!kWide) {
+      if constexpr (!(SINGLE && kWide)) {
         s.up(now.y, y_kept);
         if (outs) s.up(now.dh, dh_kept);
+      }
+      if constexpr (!SINGLE) {
+        const BackwardArgsAt a = read_again(args);
+        fold_rows<STREAM, kFold, 1>(s, a->grad_outs, a->n_out, row * a->grad_out_bytes, dh_kept);
+        fold_rows<STREAM, kFold, 1>(s, a->ins, a->n_in, row * a->in_bytes, y_kept);
       }
       if constexpr (!(SINGLE && kWide)) {
         s.mask(y_kept);
@@ -806,7 +805,7 @@ template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, h
         typedef std::integral_constant<bool, kSingle> Single;                                                                    \
         if (stream_in) bias ? run(Single{}, std::true_type{}, std::true_type{}) : run(Single{}, std::false_type{}, std::true_type{}); \
         else bias ? run(Single{}, std::true_type{}, std::false_type{}) : run(Single{}, std::false_type{}, std::false_type{});   \
-      } else if constexpr (E > 4) { /* (one pack of binary32 only with a row ahead) */                                          \
+      } else {                                                                                                                  \
         typedef std::integral_constant<bool, !kSingle> Streams; /* (16-bit rows of several gradients: 85 against 88 us, not worth a variant) */ \
         if (stream_in) bias ? run(std::false_type{}, std::true_type{}, Streams{}) : run(std::false_type{}, std::false_type{}, Streams{}); \
         else bias ? run(std::false_type{}, std::true_type{}, std::false_type{}) : run(std::false_type{}, std::false_type{}, std::false_type{}); \
