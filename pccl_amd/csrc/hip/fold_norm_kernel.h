@@ -784,9 +784,11 @@ template <int DT, bool PF32> hipError_t launch_fold_norm_sums(unsigned grid_y, h
       constexpr int E = decltype(e)::value;                                                                                     \
       constexpr int kMany = DT == PCCL_F32 && E == 16 ? 2 : 8; /* eight inputs of 64 bytes a lane would spill */                \
       const dim3 grid(n.workgroups(a.rows - a.row0)), block(n.block());                                                         \
-      if (a.n_in <= 2) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, 2, false>), grid, block, 0, stream, a);          \
-      else if (stream_in) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, kMany, true>), grid, block, 0, stream, a);    \
-      else hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, kMany, false>), grid, block, 0, stream, a);                  \
+      if constexpr (DT != PCCL_F32 || TEAM || E == 4) { /* (two packs of binary32 in one wavefront: only backward) */           \
+        if (a.n_in <= 2) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, 2, false>), grid, block, 0, stream, a);        \
+        else if (stream_in) hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, kMany, true>), grid, block, 0, stream, a);  \
+        else hipLaunchKernelGGL((fold_norm_kernel<DT, PF32, TEAM, E, kMany, false>), grid, block, 0, stream, a);                \
+      }                                                                                                                         \
     });                                                                                                                         \
     return hipGetLastError();                                                                                                   \
   }                                                                                                                             \
