@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "fold_norm_device.h"
+#include "pieces.h"
 
 using pccl_host::fail;
 
@@ -660,9 +661,7 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
   a.row_head = src_head_stride * es;
   a.n_slots = (unsigned long)(c->n_pages * c->page_tokens);
   const bool stream_in = (double)c->heads * c->head_dim * es * tokens * c->n_tensors >= (double)(48l << 20);  // (up to 2^68)
-  const long most = launch_tokens(a);
-  for (long lo = 0; lo < tokens; lo += most) {
-    const long n = std::min(most, tokens - lo);
+  return pccl_host::in_pieces(tokens, launch_tokens(a), [&](long lo, long n) {
     for (int k = 0; k < c->n_tensors; ++k) a.srcs[k] = (const char *)srcs[k] + lo * (long)a.src_token;
     a.slots = slots + lo;
     a.tokens = (unsigned)n;
@@ -674,10 +673,8 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
         else hipLaunchKernelGGL((cache_write_kernel<DT, FMT, TIMES, PARTS, false>), grid, dim3(kBlock), 0, (hipStream_t)stream, a);
       });
     });
-    rc = launched("cache_write");
-    if (rc != PCCL_OK) return rc;
-  }
-  return PCCL_OK;
+    return launched("cache_write");
+  });
 }
 
 extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *const *outs, long out_token_stride, long out_head_stride,
@@ -715,23 +712,18 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
   a.lengths = lengths;
   a.row_start = row_start;
   a.n_pages = c->n_pages;
-  const long most = launch_tokens(a);
-  for (int seq = 0; seq < n_seq; seq += 65535) {
-    a.seq0 = seq;
-    const int seqs = std::min(65535, n_seq - seq);
-    for (long lo = 0; lo < max_len; lo += most) {
+  return pccl_host::in_pieces(n_seq, 65535, [&](long seq, long seqs) {
+    a.seq0 = (int)seq;
+    return pccl_host::in_pieces(max_len, launch_tokens(a), [&](long lo, long n) {
       a.token0 = (unsigned)lo;
-      const long n = std::min(most, max_len - lo);
       with_types(dtype, c->format, [&](auto t, auto f) {
         with_shape<kReadTimes>(many((n + a.group - 1) / a.group * a.chunks.d * seqs * c->n_tensors, kReadTimes), a.parts, [&](auto times, auto parts) {
           constexpr int DT = decltype(t)::value, FMT = decltype(f)::value, TIMES = decltype(times)::value, PARTS = decltype(parts)::value;
-          hipLaunchKernelGGL((cache_read_kernel<DT, FMT, TIMES, PARTS>), dim3(workgroups(a, n, TIMES), seqs, c->n_tensors), dim3(kBlock), 0,
+          hipLaunchKernelGGL((cache_read_kernel<DT, FMT, TIMES, PARTS>), dim3(workgroups(a, n, TIMES), (unsigned)seqs, c->n_tensors), dim3(kBlock), 0,
                              (hipStream_t)stream, a);
         });
       });
-      rc = launched("cache_read");
-      if (rc != PCCL_OK) return rc;
-    }
-  }
-  return PCCL_OK;
+      return launched("cache_read");
+    });
+  });
 }
