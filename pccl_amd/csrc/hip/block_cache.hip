@@ -712,9 +712,12 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
   a.lengths = lengths;
   a.row_start = row_start;
   a.n_pages = c->n_pages;
+  // (no wavefronts for tokens that the table has no page for: max_len may be any upper bound, with row_start up to 2^31 - 1 tokens of
+  // every sequence, and those would be 2^29 wavefronts a sequence with nothing to do)
+  const long tokens = pccl_host::tokens_in_pages(max_len, table_stride, c->page_tokens);
   return pccl_host::in_pieces(n_seq, 65535, [&](long seq, long seqs) {
     a.seq0 = (int)seq;
-    return pccl_host::in_pieces(max_len, launch_tokens(a), [&](long lo, long n) {
+    return pccl_host::in_pieces(tokens, launch_tokens(a), [&](long lo, long n) {
       a.token0 = (unsigned)lo;
       with_types(dtype, c->format, [&](auto t, auto f) {
         with_shape<kReadTimes>(many((n + a.group - 1) / a.group * a.chunks.d * seqs * c->n_tensors, kReadTimes), a.parts, [&](auto times, auto parts) {

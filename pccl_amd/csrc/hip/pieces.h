@@ -16,4 +16,9 @@ int in_pieces(long total, long most, F &&f) {
   return 0;
 }
 
+// Tokens of a sequence, `most` of them at most, that `entries` pages of `page_tokens` have room for; entries may be anything from 0.
+inline long tokens_in_pages(long most, long entries, long page_tokens) {
+  return entries > most / page_tokens ? most : entries * page_tokens;
+}
+
 }  // namespace pccl_host

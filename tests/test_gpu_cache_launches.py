@@ -68,3 +68,30 @@ def test_read_of_more_tokens_than_a_launch(hip, boundary):
             p = int(table[0, t // page])
             want[row] = ref.decode("i8", codes[p, t % page], scales[p, t % page], 1, "f32")[:, 0]
     assert ref.same(out, want)
+
+
+@pytest.mark.parametrize("stride", [3, 7])
+def test_read_under_a_bound_far_beyond_the_tables(hip, stride):
+    """max_len as no bound at all: what has no page in the table takes no part in the launch."""
+    import torch
+    gen = torch.Generator().manual_seed(4)
+    n_seq, heads, dim, page, pages = 300, 2, 40, 5, 11
+    codes = torch.randint(0, 256, (pages, page, heads, dim), generator=gen, dtype=torch.uint8)
+    scales = torch.randint(100, 150, (pages, page, heads, 2), generator=gen, dtype=torch.uint8)
+    table = torch.randint(0, pages, (n_seq, stride), generator=gen, dtype=torch.int32)
+    lengths = torch.randint(0, stride * page + 1, (n_seq,), generator=gen, dtype=torch.int32)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.long().cumsum(0)])
+    rows = int(starts[-1])
+    lengths[-1] = 2 ** 31 - 1  # (tokens behind the last page are not read; those that there are are the last rows)
+    rows += stride * page - (rows - int(starts[-2]))
+    out = torch.full((rows + 2, heads, dim), -7.0, device="cuda")
+    hip.Cache("i8", heads, dim, page, pages, [codes.cuda()], [scales.cuda()]).read(
+        "f32", [out], table.cuda(), lengths.cuda(), n_seq, 2 ** 31 - 1, row_start=starts[:-1].cuda(), out_rows=rows + 2,
+        stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    want = torch.full((rows + 2, heads, dim), -7.0)
+    values = ref.decode("i8", codes, scales, dim, "f32")
+    for s in range(n_seq):
+        n = min(int(lengths[s]), stride * page)
+        want[int(starts[s]):int(starts[s]) + n] = values[table[s].long()].flatten(0, 1)[:n]
+    assert ref.same(out, want)

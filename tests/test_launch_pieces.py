@@ -24,6 +24,10 @@ int main(int argc, char **argv) {
     });
     printf("%d %ld %d\n", rc, pieces, next == total);
   }
+  const long tokens[][4] = {{0, 5, 16, 0}, {8, 0, 16, 0}, {80, 5, 16, 80}, {79, 5, 16, 79}, {81, 5, 16, 80}, {INT_MAX, 5, 16, 80}, {15, 1, 16, 15},
+                            {INT_MAX, LONG_MAX, 1 << 20, INT_MAX}, {INT_MAX, INT_MAX, 1, INT_MAX}, {INT_MAX, 2047, 1 << 20, 2047l << 20}, {INT_MAX, 2048, 1 << 20, INT_MAX}};
+  for (auto &t : tokens)
+    if (pccl_host::tokens_in_pages(t[0], t[1], t[2]) != t[3]) return 2;
   return pccl_host::in_pieces(10, 3, [](long first, long) { return first == 3 ? 7 : first > 3 ? 8 : 0; }) == 7 ? 0 : 1;
 }
 '''
