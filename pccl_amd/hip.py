@@ -345,6 +345,12 @@ class Cache:
         row, blocks = self.row_bytes(fmt, head_dim)
         d.code_page, d.code_token, d.code_head = code_strides or (page_tokens * heads * row, heads * row, row)
         d.scale_page, d.scale_token, d.scale_head = scale_strides or (page_tokens * heads * blocks, heads * blocks, blocks)
+        # (ctypes drops the bits that a field has no room for: 2^32 + 8 heads would be 8)
+        for name, given in (("heads", heads), ("head_dim", head_dim), ("page_tokens", page_tokens), ("n_pages", n_pages),
+                            *zip(("code_page", "code_token", "code_head"), code_strides or ()),
+                            *zip(("scale_page", "scale_token", "scale_head"), scale_strides or ())):
+            if getattr(d, name) != given:
+                raise PcclError(ERR_INVALID_ARG, "%s %d does not fit its field" % (name, given))
 
     @staticmethod
     def row_bytes(fmt, head_dim):
@@ -380,6 +386,8 @@ class Cache:
             if not hasattr(page_table, "shape"):
                 raise PcclError(ERR_INVALID_ARG, "table_stride is needed where the page table cannot tell it")
             table_stride = page_table.shape[-1]
+        if n_seq > 0x7fffffff:  # (ctypes would drop the bits above)
+            raise PcclError(ERR_INVALID_ARG, "n_seq %d outside [0, 2^31)" % n_seq)
         if out_rows is None:
             if row_start is not None:
                 raise PcclError(ERR_INVALID_ARG, "row_start without out_rows")
