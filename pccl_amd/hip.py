@@ -7,6 +7,7 @@ code, carrying the library's error text.
 import ctypes
 import os
 import struct
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libpccl_hip.so")
@@ -233,15 +234,67 @@ def _at(x):
         return int(x)
 
 
-def _many(x, most, what):
-    """Addresses of a list of operands, padded to the fixed array that they go to."""
-    if len(x) > most:
-        raise PcclError(ERR_INVALID_ARG, "%d %s, at most %d" % (len(x), what, most))
+# Element types as torch names them
+_TORCH = {F32: "float32", I32: "int32", BF16: "bfloat16", F16: "float16", F8E4M3: "float8_e4m3fn", F8E5M2: "float8_e5m2", F64: "float64", U32: "uint32"}
+
+
+def _kind(code):
+    """torch's object for a dtype code; None where there is none, or no torch (nor tensors) so far."""
+    return getattr(sys.modules.get("torch"), _TORCH.get(code, ""), None)
+
+
+def _on_device(x, what):
+    """Refuses a tensor that the GPU can't reach (it would fault); pinned host memory it can."""
+    if not x.is_cuda and x.numel() and not x.is_pinned():
+        raise PcclError(ERR_INVALID_ARG, "%s: a tensor on %s, device memory is needed" % (what, x.device))
+
+
+def _check_tensor(x, code, what):
+    """Refuses a tensor of elements other than `code`'s (read as those it would be garbage, and could end before its last row) or outside of
+    the GPU's memory.  Whole numbers of the same size pass: a buffer of raw bits.  Operands that are no tensors are taken at their word."""
+    kind, torch = getattr(x, "dtype", None), sys.modules.get("torch")
+    if torch is None or not isinstance(kind, torch.dtype):
+        return
+    if code in ELEM_BYTES and kind is not _kind(code) and (kind.is_floating_point or kind.is_complex or x.element_size() != ELEM_BYTES[code]):
+        raise PcclError(ERR_INVALID_ARG, "%s: elements are %s, not %s" % (what, kind, _TORCH[code]))
+    _on_device(x, what)
+
+
+def _typed(x, kind, code, what):
+    """Address of an operand with elements of dtype `code`, 0 for none."""
+    if x is None:
+        return 0
     try:
-        at = [t.data_ptr() for t in x]  # (all of them tensors: half the time of asking each)
+        if x.dtype is not kind or not x.is_cuda:
+            _check_tensor(x, code, what)
+        return x.data_ptr()
     except AttributeError:
-        at = [_at(t) for t in x]
-    return at + _ZEROS[:most - len(x)]
+        return _at(x)
+
+
+def _many(x, most, kind, code, what):
+    """Addresses of a list of operands with elements of dtype `code`, padded to the fixed array that they go to."""
+    try:
+        at = [t.data_ptr() for t in x if t.dtype is kind and t.is_cuda]  # (all of them such tensors: half the time of asking each)
+    except AttributeError:
+        at = ()
+    if len(at) != len(x):
+        at = [_typed(t, kind, code, what) for t in x]
+    if len(at) > most:
+        raise PcclError(ERR_INVALID_ARG, "%d %s, at most %d" % (len(at), what, most))
+    return at + _ZEROS[:most - len(at)]
+
+
+def _room(x, extent, what):
+    """Address of a buffer of `extent` bytes; of one that can tell (a torch tensor), whether its memory goes that far is checked, however
+    it is viewed."""
+    if x is not None and type(x) is not int and hasattr(x, "untyped_storage"):
+        storage, at = x.untyped_storage(), x.data_ptr()
+        room = storage.data_ptr() + storage.nbytes() - at if at else 0
+        if room < extent:
+            raise PcclError(ERR_INVALID_ARG, "%s: %d bytes, %d are needed" % (what, room, extent))
+        _on_device(x, what)
+    return _at(x)
 
 
 def _index(x, itemsize, count, what):
@@ -251,14 +304,8 @@ def _index(x, itemsize, count, what):
             raise PcclError(ERR_INVALID_ARG, "%s: %d entries of %d bytes, %d of %d are needed" % (what, x.numel(), x.element_size(), count, itemsize))
         if not x.is_contiguous():  # (an expanded one has fewer entries in memory than it counts)
             raise PcclError(ERR_INVALID_ARG, "%s: entries must lie side by side" % what)
+        _on_device(x, what)
     return _at(x)
-
-
-def _packed(layout, *values):
-    try:
-        return layout.pack(*values)
-    except struct.error as e:  # a number that its field cannot hold
-        raise PcclError(ERR_INVALID_ARG, str(e)) from None
 
 
 class FoldNorm:
@@ -276,22 +323,36 @@ class FoldNorm:
         self.width = width
         self._params = (post_weight, post_bias, pre_weight, pre_bias)
         dtype = _code(DTYPES, dtype)
-        self._settings = (dtype, dtype if param_dtype is None else _code(DTYPES, param_dtype), _code(NORMS, post), _code(NORMS, pre),
+        params = dtype if param_dtype is None else _code(DTYPES, param_dtype)
+        for x, what in zip(self._params, ("post_weight", "post_bias", "pre_weight", "pre_bias")):
+            if x is not None and hasattr(x, "is_contiguous") and (x.numel() < width or not x.is_contiguous()):
+                raise PcclError(ERR_INVALID_ARG, "%s: %d elements side by side are needed" % (what, width))
+            _check_tensor(x, params, what)
+        self._rows, self._vectors = (_kind(dtype), dtype), (_kind(params), params)
+        self._settings = (dtype, params, _code(NORMS, post), _code(NORMS, pre),
                           *(ctypes.c_float(x).value for x in (post_eps, pre_eps, weight_offset, residual_scale, block_scale)))
 
     def _desc(self, ins, n_out, rows, gate, gate_rows, gate_stride, in_stride, residual, residual_stride, residual_out, residual_out_stride,
               folded, folded_stride, outs, out_stride):
-        w = self.width
-        return _packed(_FOLD_NORM_DESC, *self._settings, len(ins), n_out, 0, rows, w, *[_at(x) for x in self._params],
-                       _at(gate), w if gate_stride is None else gate_stride, gate_rows, *_many(ins, MAX_INPUTS, "inputs"),
-                       w if in_stride is None else in_stride, _at(residual), w if residual_stride is None else residual_stride,
-                       _at(residual_out), w if residual_out_stride is None else residual_out_stride, _at(folded),
-                       w if folded_stride is None else folded_stride, *_many(outs, MAX_OUTPUTS, "outputs"), w if out_stride is None else out_stride)
+        w, (kind, code), (p0, p1, p2, p3) = self.width, self._rows, self._params
+        try:
+            return _FOLD_NORM_DESC.pack(
+                *self._settings, len(ins), n_out, 0, rows, w, 0 if p0 is None else _at(p0), 0 if p1 is None else _at(p1),
+                0 if p2 is None else _at(p2), 0 if p3 is None else _at(p3), 0 if gate is None else _typed(gate, *self._vectors, "gate"),
+                w if gate_stride is None else gate_stride, gate_rows, *_many(ins, MAX_INPUTS, kind, code, "inputs"),
+                w if in_stride is None else in_stride, 0 if residual is None else _typed(residual, kind, code, "residual"),
+                w if residual_stride is None else residual_stride, 0 if residual_out is None else _typed(residual_out, kind, code, "residual_out"),
+                w if residual_out_stride is None else residual_out_stride, 0 if folded is None else _typed(folded, kind, code, "folded"),
+                w if folded_stride is None else folded_stride, *(_many(outs, MAX_OUTPUTS, kind, code, "outputs") if outs else _ZEROS),
+                w if out_stride is None else out_stride)
+        except struct.error as e:  # a number that its field cannot hold
+            raise PcclError(ERR_INVALID_ARG, str(e)) from None
 
     def forward(self, ins, outs, rows, residual=None, residual_out=None, folded=None, gate=None, gate_rows=0, stream=None,
                 in_stride=None, residual_stride=None, residual_out_stride=None, folded_stride=None, gate_stride=None, out_stride=None):
         """h to every buffer of `outs` (none: h is not computed), r to `residual_out`, y to `folded`, where given.  The gate
-        has one row for every `gate_rows` rows.  Strides in elements from row to row, by default the width."""
+        has one row for every `gate_rows` rows.  Strides in elements from row to row, by default the width.  Of a torch tensor the element type
+        is checked; how far it goes is up to the caller, as with reduce_copy."""
         d = self._desc(ins, len(outs), rows, gate, gate_rows, gate_stride, in_stride, residual, residual_stride, residual_out,
                        residual_out_stride, folded, folded_stride, outs, out_stride)
         _check(lib().pccl_hip_fold_norm(d, _at(stream)))
@@ -311,17 +372,22 @@ class FoldNorm:
         further on.  Written where given: grad_ins (each the gradient of y), grad_residual, grad_gate and those of the
         parameters.  workspace: a buffer of workspace_bytes(rows, gate_rows), its size taken from the buffer where it can
         tell (a torch tensor), else from the argument."""
-        w = self.width
+        w, (kind, code), vectors = self.width, self._rows, self._vectors
         d = self._desc(ins, len(grad_outs), rows, gate, gate_rows, gate_stride, in_stride, None, None, residual_out, residual_out_stride, None, None,
                        (), None)
         if workspace is not None and workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
-        g = _packed(_FOLD_NORM_GRADS, *_many(grad_outs, MAX_OUTPUTS, "gradients of the outputs"), w if grad_out_stride is None else grad_out_stride,
-                    _at(grad_residual_out), w if grad_residual_out_stride is None else grad_residual_out_stride,
-                    *_many(grad_ins, MAX_INPUTS, "gradients of the inputs"), len(grad_ins), 0, w if grad_in_stride is None else grad_in_stride,
-                    _at(grad_residual), w if grad_residual_stride is None else grad_residual_stride,
-                    _at(grad_gate), w if grad_gate_stride is None else grad_gate_stride, _at(grad_post_weight), _at(grad_post_bias),
-                    _at(grad_pre_weight), _at(grad_pre_bias), _at(workspace), workspace_bytes or 0)
+        try:
+            g = _FOLD_NORM_GRADS.pack(
+                *_many(grad_outs, MAX_OUTPUTS, kind, code, "gradients of the outputs"), w if grad_out_stride is None else grad_out_stride,
+                _typed(grad_residual_out, kind, code, "grad_residual_out"), w if grad_residual_out_stride is None else grad_residual_out_stride,
+                *_many(grad_ins, MAX_INPUTS, kind, code, "gradients of the inputs"), len(grad_ins), 0, w if grad_in_stride is None else grad_in_stride,
+                _typed(grad_residual, kind, code, "grad_residual"), w if grad_residual_stride is None else grad_residual_stride,
+                _typed(grad_gate, *vectors, "grad_gate"), w if grad_gate_stride is None else grad_gate_stride,
+                _typed(grad_post_weight, *vectors, "grad_post_weight"), _typed(grad_post_bias, *vectors, "grad_post_bias"),
+                _typed(grad_pre_weight, *vectors, "grad_pre_weight"), _typed(grad_pre_bias, *vectors, "grad_pre_bias"), _at(workspace), workspace_bytes or 0)
+        except struct.error as e:
+            raise PcclError(ERR_INVALID_ARG, str(e)) from None
         _check(lib().pccl_hip_fold_norm_backward(d, g, _at(stream)))
 
 
@@ -338,8 +404,8 @@ class Cache:
         d.heads, d.head_dim, d.page_tokens, d.n_pages = heads, head_dim, page_tokens, n_pages
         if len(codes) != len(scales):
             raise PcclError(ERR_INVALID_ARG, "%d tensors of codes, %d of scales" % (len(codes), len(scales)))
-        d.codes[:] = _many(codes, CACHE_MAX_TENSORS, "tensors of codes")
-        d.scales[:] = _many(scales, CACHE_MAX_TENSORS, "tensors of scales")
+        if len(codes) > CACHE_MAX_TENSORS:
+            raise PcclError(ERR_INVALID_ARG, "%d tensors, at most %d" % (len(codes), CACHE_MAX_TENSORS))
         d.n_tensors = self.n_tensors = len(codes)
         self._ref, self._array = ctypes.byref(d), ctypes.c_void_p * self.n_tensors  # (the description is only read from here on)
         row, blocks = self.row_bytes(fmt, head_dim)
@@ -351,6 +417,11 @@ class Cache:
                             *zip(("scale_page", "scale_token", "scale_head"), scale_strides or ())):
             if getattr(d, name) != given:
                 raise PcclError(ERR_INVALID_ARG, "%s %d does not fit its field" % (name, given))
+        counts = (n_pages, page_tokens, heads)
+        for to, buffers, strides, last, what in ((d.codes, codes, (d.code_page, d.code_token, d.code_head), row, "codes"),
+                                                 (d.scales, scales, (d.scale_page, d.scale_token, d.scale_head), blocks, "scales")):
+            extent = last + sum((n - 1) * stride for n, stride in zip(counts, strides)) if min(counts) > 0 else 0
+            to[:] = [_room(x, extent, what) for x in buffers] + _ZEROS[:CACHE_MAX_TENSORS - len(buffers)]
 
     @staticmethod
     def row_bytes(fmt, head_dim):
@@ -358,19 +429,21 @@ class Cache:
         bits = 4 if _code(CACHE_FORMATS, fmt) == CACHE_F4E2M1 else 8
         return (head_dim * bits + 7) // 8, (head_dim + CACHE_BLOCK - 1) // CACHE_BLOCK
 
-    def _operands(self, x, what):
+    def _operands(self, x, code, what):
         if len(x) != self.n_tensors:
             raise PcclError(ERR_INVALID_ARG, "%d %s for %d tensors" % (len(x), what, self.n_tensors))
-        return self._array(*[_at(t) for t in x])
+        kind = _kind(code)
+        return self._array(*[_typed(t, kind, code, what) for t in x])
 
     def write(self, dtype, srcs, slots, tokens, stream=None, token_stride=None, head_stride=None):
         """Codes `tokens` rows of heads x head_dim elements of every source into slots[i] = page * page_tokens + token of the page
         (int64 on the device, side by side; a slot outside the cache: the row is left out).  The slots of one call must differ.  Strides in
         elements, by default those of a dense [tokens, heads, head_dim]."""
-        srcs = self._operands(srcs, "sources")
+        dtype = _code(DTYPES, dtype)
+        srcs = self._operands(srcs, dtype, "sources")
         head_stride = self.head_dim if head_stride is None else head_stride
         token_stride = self.heads * self.head_dim if token_stride is None else token_stride
-        _check(lib().pccl_hip_cache_write(self._ref, _code(DTYPES, dtype), srcs, token_stride, head_stride,
+        _check(lib().pccl_hip_cache_write(self._ref, dtype, srcs, token_stride, head_stride,
                                           _index(slots, 8, tokens, "slots"), tokens, _at(stream)))
 
     def read(self, dtype, outs, page_table, lengths, n_seq, max_len, row_start=None, out_rows=None, table_stride=None, stream=None,
@@ -379,7 +452,8 @@ class Cache:
         `out_rows` rows), or without row_start to row s * max_len + t.  page_table, lengths (int32) and row_start (int64) are on
         the device, their entries side by side; table_stride, the entries of a sequence, is by default what a dense 2-d table says.  Rows that no token goes to
         are left as they are."""
-        outs = self._operands(outs, "outputs")
+        dtype = _code(DTYPES, dtype)
+        outs = self._operands(outs, dtype, "outputs")
         head_stride = self.head_dim if head_stride is None else head_stride
         token_stride = self.heads * self.head_dim if token_stride is None else token_stride
         if table_stride is None:
@@ -392,7 +466,7 @@ class Cache:
             if row_start is not None:
                 raise PcclError(ERR_INVALID_ARG, "row_start without out_rows")
             out_rows = n_seq * max_len
-        _check(lib().pccl_hip_cache_read(self._ref, _code(DTYPES, dtype), outs, token_stride, head_stride, out_rows,
+        _check(lib().pccl_hip_cache_read(self._ref, dtype, outs, token_stride, head_stride, out_rows,
                                          _index(page_table, 4, n_seq * table_stride, "page_table"), table_stride,
                                          _index(lengths, 4, n_seq, "lengths"), _index(row_start, 8, n_seq, "row_start"), n_seq, max_len,
                                          _at(stream)))
