@@ -375,8 +375,13 @@ class FoldNorm:
         w, (kind, code), vectors = self.width, self._rows, self._vectors
         d = self._desc(ins, len(grad_outs), rows, gate, gate_rows, gate_stride, in_stride, None, None, residual_out, residual_out_stride, None, None,
                        (), None)
-        if workspace is not None and workspace_bytes is None:
-            workspace_bytes = workspace.numel() * workspace.element_size()
+        if workspace is not None and type(workspace) is not int and hasattr(workspace, "element_size"):
+            _on_device(workspace, "workspace")
+            room = workspace.numel() * workspace.element_size()
+            if workspace_bytes is None:
+                workspace_bytes = room
+            elif workspace_bytes > room:
+                raise PcclError(ERR_INVALID_ARG, "workspace_bytes %d of a buffer of %d" % (workspace_bytes, room))
         try:
             g = _FOLD_NORM_GRADS.pack(
                 *_many(grad_outs, MAX_OUTPUTS, kind, code, "gradients of the outputs"), w if grad_out_stride is None else grad_out_stride,

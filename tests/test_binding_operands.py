@@ -115,3 +115,12 @@ def test_host_memory():
                  lambda: c.read("bf16", [A], table, A, 1, 8), lambda: c.read("bf16", [A], A, lengths, 1, 8, table_stride=4),
                  lambda: c.read("bf16", [A], A, A, 1, 8, table_stride=4, row_start=slots, out_rows=8)):
         assert "device memory" in refused(call)
+
+
+def test_workspace():
+    n = hip.FoldNorm("bf16", 64, pre_weight=A)
+    back = lambda **kw: n.backward([A], [A], [A], 2, residual_out=A, grad_pre_weight=A, **kw)  # noqa: E731
+    assert "workspace of 0 bytes" in refused(back, workspace=A)  # (an address can't tell its size)
+    assert "workspace of 16 bytes" in refused(back, workspace=A, workspace_bytes=16)
+    assert "device memory" in refused(back, workspace=tensors("uint8", 1 << 20))
+    assert "of a buffer of 0" in refused(back, workspace=tensors("uint8", 0), workspace_bytes=1 << 20)
