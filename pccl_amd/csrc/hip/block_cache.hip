@@ -654,7 +654,7 @@ extern "C" int pccl_hip_cache_write(const pccl_cache_desc *c, int dtype, const v
   if (tokens && !slots) return fail(PCCL_ERR_INVALID_ARG, "slots are null");
   for (int k = 0; k < c->n_tensors; ++k)
     if (tokens && !srcs[k]) return fail(PCCL_ERR_INVALID_ARG, "source %d is null", k);
-  rc = pccl_host::check_stream(stream);
+  rc = pccl_host::check_stream(&stream);
   if (rc != PCCL_OK) return rc;
   if (tokens == 0 || c->n_pages == 0) return PCCL_OK;
   a.src_token = (unsigned)(src_token_stride * es);
@@ -700,7 +700,7 @@ extern "C" int pccl_hip_cache_read(const pccl_cache_desc *c, int dtype, void *co
   if (!nothing && (!page_table || !lengths)) return fail(PCCL_ERR_INVALID_ARG, "page_table or lengths are null");
   for (int k = 0; k < c->n_tensors; ++k)
     if (!nothing && !outs[k]) return fail(PCCL_ERR_INVALID_ARG, "output %d is null", k);
-  rc = pccl_host::check_stream(stream);
+  rc = pccl_host::check_stream(&stream);
   if (rc != PCCL_OK || nothing) return rc;
   for (int k = 0; k < c->n_tensors; ++k) a.outs[k] = (char *)outs[k];
   a.out_token = (unsigned)(out_token_stride * es);

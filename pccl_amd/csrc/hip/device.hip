@@ -72,8 +72,12 @@ int executor_id() { return g_executor_id.load(std::memory_order_relaxed); }
 static std::atomic<long> g_slice_bytes{32l << 30};
 long slice_bytes() { return g_slice_bytes.load(std::memory_order_relaxed); }
 
-int check_stream(void *stream) {
-  if (!stream) return PCCL_OK;
+int check_stream(void **given) {
+  // The default streams' handles are small numbers, not addresses, and mean the current device's; hipStreamGetDevice follows hipStreamLegacy
+  // as an address.  That one is the null stream by another name.
+  if (*given == (void *)hipStreamLegacy) *given = nullptr;
+  void *const stream = *given;
+  if (!stream || stream == (void *)hipStreamPerThread) return PCCL_OK;
   hipDevice_t of = 0;
   int current = 0;
   PCCL_HIP_CHECK(hipGetDevice(&current));

@@ -176,7 +176,7 @@ extern "C" int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream) {
     c.out(d->outs[j], d->out_stride, "an output", d->rows, c.es);
   }
   if (c.rc != PCCL_OK) return c.rc;
-  rc = pccl_host::check_stream(stream);
+  rc = pccl_host::check_stream(&stream);
   if (rc != PCCL_OK) return rc;
   if (d->rows == 0) return PCCL_OK;
   ForwardArgs a;
@@ -262,7 +262,7 @@ extern "C" int pccl_hip_fold_norm_backward(const pccl_fold_norm_desc *d, const p
       return fail(PCCL_ERR_INVALID_ARG, "workspace of %ld bytes, %ld are needed", g->workspace ? g->workspace_bytes : 0, need);
     if ((uintptr_t)g->workspace % 16) return fail(PCCL_ERR_MISALIGNED, "workspace (%p) not 16-byte aligned", g->workspace);
   }
-  rc = pccl_host::check_stream(stream);
+  rc = pccl_host::check_stream(&stream);
   if (rc != PCCL_OK) return rc;
   if (d->rows == 0 && !any) return PCCL_OK;
 

@@ -36,8 +36,9 @@ struct Tuning {
 };
 Tuning tuning();
 
-// PCCL_OK if `stream` (null: the default stream) belongs to the calling thread's current device, else an error code.
-int check_stream(void *stream);
+// PCCL_OK if the stream (null, hipStreamLegacy, hipStreamPerThread: the default streams) belongs to the calling thread's current
+// device, else an error code; hipStreamLegacy is replaced by null.
+int check_stream(void **stream);
 
 // Longest stretch of an operand, in bytes, that one launch of pccl_hip_reduce_copy / pccl_hip_accumulate
 // covers (a multiple of 4 KiB; see pccl_hip_set_slice_bytes).

@@ -124,3 +124,13 @@ def test_workspace():
     assert "workspace of 16 bytes" in refused(back, workspace=A, workspace_bytes=16)
     assert "device memory" in refused(back, workspace=tensors("uint8", 1 << 20))
     assert "of a buffer of 0" in refused(back, workspace=tensors("uint8", 0), workspace_bytes=1 << 20)
+
+
+@pytest.mark.parametrize("stream", [0, 1, 2])
+def test_default_streams(stream):
+    """The default streams' handles (null, hipStreamLegacy, hipStreamPerThread) are no addresses: nothing is asked about them."""
+    hip.FoldNorm("bf16", 64).forward([A], [A], 0, stream=stream)
+    hip.FoldNorm("bf16", 64).backward([A], [A], [A], 0, residual_out=A, stream=stream)
+    c = hip.Cache("i8", 1, 32, 1, 1, [A], [A])
+    c.write("bf16", [A], A, 0, stream=stream)
+    c.read("bf16", [A], A, A, 0, 8, table_stride=1, stream=stream)
