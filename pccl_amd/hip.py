@@ -343,7 +343,7 @@ class FoldNorm:
                 w if in_stride is None else in_stride, 0 if residual is None else _typed(residual, kind, code, "residual"),
                 w if residual_stride is None else residual_stride, 0 if residual_out is None else _typed(residual_out, kind, code, "residual_out"),
                 w if residual_out_stride is None else residual_out_stride, 0 if folded is None else _typed(folded, kind, code, "folded"),
-                w if folded_stride is None else folded_stride, *(_many(outs, MAX_OUTPUTS, kind, code, "outputs") if outs else _ZEROS),
+                w if folded_stride is None else folded_stride, *(_many(outs, MAX_OUTPUTS, kind, code, "outputs") if len(outs) else _ZEROS),
                 w if out_stride is None else out_stride)
         except struct.error as e:  # a number that its field cannot hold
             raise PcclError(ERR_INVALID_ARG, str(e)) from None

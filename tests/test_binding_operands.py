@@ -134,3 +134,17 @@ def test_default_streams(stream):
     c = hip.Cache("i8", 1, 32, 1, 1, [A], [A])
     c.write("bf16", [A], A, 0, stream=stream)
     c.read("bf16", [A], A, A, 0, 8, table_stride=1, stream=stream)
+
+
+def test_operands_stacked_in_one_tensor():
+    """A tensor of partial outputs, copies or caches stands for the list of its first dimension."""
+    two = tensors("bfloat16", 2, 0)
+    n = hip.FoldNorm("bf16", 64, post="rms")
+    n.forward(two, two, 0)
+    n.backward(two, two, two, 0, residual_out=two[0])
+    refused(n.forward, tensors("float32", 2, 0), two, 0)
+    refused(n.forward, two, tensors("bfloat16", 9, 0), 0)
+    raw = tensors("uint8", 2, 0)
+    c = hip.Cache("i8", 1, 32, 1, 0, raw, raw)
+    c.write("bf16", two, A, 0)
+    c.read("bf16", two, A, A, 0, 8, table_stride=1)
