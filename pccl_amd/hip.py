@@ -371,7 +371,8 @@ class FoldNorm:
         the forward pass; grad_outs: the partial gradients of h, folded here; grad_residual_out: the gradient of r from
         further on.  Written where given: grad_ins (each the gradient of y), grad_residual, grad_gate and those of the
         parameters.  workspace: a buffer of workspace_bytes(rows, gate_rows), its size taken from the buffer where it can
-        tell (a torch tensor), else from the argument."""
+        tell (a torch tensor), else from the argument; no reference is kept, and it must live until the work on `stream` is done
+        (torch: record_stream, or keep it)."""
         w, (kind, code), vectors = self.width, self._rows, self._vectors
         d = self._desc(ins, len(grad_outs), rows, gate, gate_rows, gate_stride, in_stride, None, None, residual_out, residual_out_stride, None, None,
                        (), None)
