@@ -153,7 +153,8 @@ int pccl_hip_set_rotation(int rotate);
  * where an absent weight (NULL) counts as factor 1 (weight_offset is then not added) and an absent bias as 0.
  * x is absent (residual == NULL: 0) or given; g is absent (gate == NULL: 1) or row i / gate_rows of the gate.
  * Statistics are held in binary32; a row whose sum of squares passes the largest binary32 is outside of
- * what the norms can do.  No counterpart in the reference, which has no model-side code; the fold and the store to
+ * what the norms can do, and a layer norm's mean carries the rounding of a binary32 sum (below 2^-18 of the row's mean magnitude):
+ * elements that differ by no more than that are told apart no better.  No counterpart in the reference, which has no model-side code; the fold and the store to
  * every output are those of multimem_ld_reduce and multimemStore (utils/multimem.h:12-102). */
 enum pccl_norm_kind { PCCL_NORM_NONE = 0, PCCL_NORM_RMS = 1, PCCL_NORM_LAYER = 2 };
 #define PCCL_NORM_MAX_WIDTH 16384
@@ -199,7 +200,9 @@ int pccl_hip_fold_norm(const pccl_fold_norm_desc *d, void *stream);
  *   grad_gate          sums of block_scale * dr * n over the rows that share a gate row
  *   grad_*_weight / grad_*_bias  sums over all rows
  * Statistics are computed again from y and r.  Sums over rows are held in binary32 and added in a fixed order: the same call
- * gives the same bits.  Every pointer may be NULL: the gradient is then not computed, or taken as zero. */
+ * gives the same bits.  grad_residual_out may be NULL (zero), and so may each of grad_residual, grad_gate and the parameters' gradients
+ * (not computed).  The n_in ins, n_out grad_outs and n_grad_in grad_ins are all given, ins also where neither a post norm nor a
+ * gate's gradient needs y; a gradient that is not there is left out of its count. */
 typedef struct pccl_fold_norm_grads {
   const void *grad_outs[PCCL_MAX_OUTPUTS];
   long grad_out_stride;
@@ -214,7 +217,7 @@ typedef struct pccl_fold_norm_grads {
   void *grad_gate;
   long grad_gate_stride;
   void *grad_post_weight, *grad_post_bias, *grad_pre_weight, *grad_pre_bias;
-  void *workspace;           /* pccl_hip_fold_norm_workspace bytes, 16-byte aligned; used while the launches run */
+  void *workspace;           /* pccl_hip_fold_norm_workspace bytes, 16-byte aligned; the launches' own until they have run */
   long workspace_bytes;
 } pccl_fold_norm_grads;
 
