@@ -247,8 +247,10 @@ struct Columns {
 // Rows beyond 8192 columns (E = 16) have sixteen wavefronts, all of a compute unit's registers, 8 for each column.  They go pack by pack,
 // in order: what a pack needs of wpre and cgw is read from the caches as it comes, y, r and dh stay as they were loaded and are unpacked and
 // centred anew in each phase, s1 and p1 are in LDS, the post norm's sums over strips go to the workspace and back, and only 16-bit rows
-// without BIAS have the next row on its way.  (2048 x 16384 bf16 113 -> 106 us, with biases 226 -> 131; f32 1024 x 16384 148 -> 105: the
-// whole row at once spilled 18 to 123 registers.)
+// without BIAS have the next row on its way.  (2048 x 16384 bf16 113 -> 106 us, with biases 226 -> 128; f32 1024 x 16384 148 -> 105, with
+// biases 212 -> 186; the floors are 59.)  They still spill, less than the whole row at once did: without BIAS 0 to 2 of 128 registers
+// for one gradient of 16-bit rows, 0 or 1 for several, 12 and 43 for binary32; with BIAS 18 to 22, 57 to 77, 98 and 132.  Of the narrower
+// instances only some with BIAS spill: two packs of binary32 5 (a team) and 13 (one wavefront), one wavefront of 16-bit rows 4 to 8.
 // BIAS: some bias's gradient or a gate behind a biased norm is asked for (s0 and p0 are kept).
 // STREAM: rows are read non-temporally.
 //
@@ -265,7 +267,7 @@ struct BackRow {
 };
 
 // Whether calls of one y and at most one dh have instances of their own: all but two packs of binary32 in one wavefront (50000 x 400
-// 98 us with and without; beyond 4096 columns 2048 x 8192 88 -> 84).
+// 98 us with and without, where 92 was reached before calls of several gradients took this form; beyond 4096 columns 2048 x 8192 88 -> 84).
 template <int DT, bool TEAM, int E>
 constexpr bool row_single() { return E == RowType<DT>::kPack || TEAM; }
 
