@@ -148,3 +148,8 @@ def test_operands_stacked_in_one_tensor():
     c = hip.Cache("i8", 1, 32, 1, 0, raw, raw)
     c.write("bf16", two, A, 0)
     c.read("bf16", two, A, A, 0, 8, table_stride=1)
+
+
+def test_codes_that_their_fields_cannot_hold():
+    refused(hip.FoldNorm, 2 ** 40, 64)
+    refused(hip.FoldNorm, "bf16", 64, post=2 ** 33)
