@@ -253,12 +253,13 @@ def _on_device(x, what):
 
 
 def _check_tensor(x, code, what):
-    """Refuses a tensor of elements other than `code`'s (read as those it would be garbage, and could end before its last row) or outside of
-    the GPU's memory.  Whole numbers of the same size pass: a buffer of raw bits.  Operands that are no tensors are taken at their word."""
+    """Refuses a tensor of numbers of another type than `code`'s (read as those they would be garbage, and could end before the last row) or
+    outside of the GPU's memory.  Whole numbers pass, whatever their size: a buffer of raw bytes.  Operands that are no tensors are taken at
+    their word."""
     kind, torch = getattr(x, "dtype", None), sys.modules.get("torch")
     if torch is None or not isinstance(kind, torch.dtype):
         return
-    if code in ELEM_BYTES and kind is not _kind(code) and (kind.is_floating_point or kind.is_complex or x.element_size() != ELEM_BYTES[code]):
+    if code in ELEM_BYTES and kind is not _kind(code) and (kind.is_floating_point or kind.is_complex):
         raise PcclError(ERR_INVALID_ARG, "%s: elements are %s, not %s" % (what, kind, _TORCH[code]))
     _on_device(x, what)
 
@@ -335,7 +336,7 @@ class FoldNorm:
         dtype = _code(DTYPES, dtype)
         params = dtype if param_dtype is None else _code(DTYPES, param_dtype)
         for x, what in zip(self._params, ("post_weight", "post_bias", "pre_weight", "pre_bias")):
-            if x is not None and hasattr(x, "is_contiguous") and (x.numel() < width or not x.is_contiguous()):
+            if x is not None and hasattr(x, "is_contiguous") and (x.numel() * x.element_size() < width * ELEM_BYTES.get(params, 0) or not x.is_contiguous()):
                 raise PcclError(ERR_INVALID_ARG, "%s: %d elements side by side are needed" % (what, width))
             _check_tensor(x, params, what)
         self._addresses = [getattr(p, "data_ptr", None) or int(p or 0).__index__ for p in self._params]  # (called anew for each call)

@@ -55,14 +55,16 @@ def test_rows_of_another_element_type():
 
 
 def test_raw_bits_and_addresses_pass():
-    raw = tensors("int16", 0)
+    raw, raw_bytes = tensors("int16", 0), tensors("uint8", 0)
 
     class Buffer:  # (says where it is, not what it holds)
         def data_ptr(self):
             return A
 
-    hip.FoldNorm("bf16", 64).forward([raw, A, Buffer()], [Buffer(), raw], 0, residual=raw)
-    refused(hip.FoldNorm("f32", 64).forward, [raw], [A], 0)
+    hip.FoldNorm("bf16", 64).forward([raw, A, Buffer()], [Buffer(), raw_bytes], 0, residual=raw)
+    hip.FoldNorm("f32", 64).forward([raw_bytes], [raw], 0)
+    assert "64 elements" in refused(hip.FoldNorm, "f32", 64, pre_weight=tensors("uint8", 255))
+    assert "device memory" in refused(hip.FoldNorm, "f32", 64, pre_weight=tensors("uint8", 256))
     refused(hip.FoldNorm("bf16", 64).forward, [tensors("float16", 0)], [A], 0)
 
 
